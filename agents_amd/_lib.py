@@ -19,6 +19,8 @@ AA_A_ROW, AA_A_COL, AA_A_PATCH, AA_A_PATCH_U8, AA_A_PATCH_T, AA_A_PATCH_T_U8 = 0
 AA_B_ROW, AA_B_COL = 0, 1
 AA_LOSS_HUBER, AA_LOSS_SQUARED, AA_LOSS_TARGETS = 0, 1, 2
 AA_OBS_U8, AA_OBS_F32 = 0, 1
+AA_DT_F32, AA_DT_BF16, AA_DT_F16 = 0, 1, 2
+AA_CATEGORICAL_MAX_TOP = 64
 AA_SAC_STD_EXP, AA_SAC_STD_CLIP_EXP = 0, 1
 AA_PPO_NSTATS = 8
 AA_PPO_DIST_STATS = 16 + 6 * 256
@@ -113,6 +115,30 @@ class PpoPolicyStepDesc(Structure):
                 ("D", c_int32), ("loc", c_void_p), ("scale", c_void_p),
                 ("seed", c_uint64), ("call_counter_dev", c_void_p), ("arrival_dev", c_void_p),
                 ("clip_lo", c_void_p), ("clip_hi", c_void_p), ("action", c_void_p)]
+
+
+class CategoricalDesc(Structure):
+    """aa_categorical_desc (include/agents_amd.h)."""
+    _fields_ = [("rows", c_int64), ("inner", c_int64), ("vocab", c_int64), ("logits", c_void_p),
+                ("x_outer", c_int64), ("x_inner", c_int64), ("actions", c_void_p),
+                ("a_outer", c_int64), ("a_inner", c_int64), ("first_action", c_int64),
+                ("mask", c_void_p), ("k_outer", c_int64), ("k_inner", c_int64),
+                ("dtype", c_int32), ("action_bytes", c_int32), ("mask_bytes", c_int32),
+                ("top_k", c_int32), ("temperature", c_float), ("log_prob", c_void_p),
+                ("entropy", c_void_p), ("stats", c_void_p), ("top_ids", c_void_p),
+                ("top_log_prob", c_void_p)]
+
+
+class LayerNormDesc(Structure):
+    """aa_layer_norm_desc (include/agents_amd.h)."""
+    _fields_ = [("rows", c_int64), ("inner", c_int64), ("width", c_int64), ("x", c_void_p),
+                ("x_outer", c_int64), ("x_inner", c_int64), ("dy", c_void_p),
+                ("dy_outer", c_int64), ("dy_inner", c_int64), ("y", c_void_p),
+                ("y_outer", c_int64), ("y_inner", c_int64), ("dx", c_void_p),
+                ("dx_outer", c_int64), ("dx_inner", c_int64), ("gamma", c_void_p),
+                ("beta", c_void_p), ("stats", c_void_p), ("dgamma", c_void_p),
+                ("dbeta", c_void_p), ("epsilon", c_float), ("dtype", c_int32),
+                ("mask_act", c_int32)]
 
 
 class MlpWideBwd(Structure):
@@ -394,6 +420,16 @@ _SIGNATURES = {
                           [c_void_p] * 3),
     "aa_sac_alpha_step": (c_int, [c_void_p] * 3 + [c_float, c_int32, c_float, c_int64, c_float] +
                           [c_void_p] * 5 + [c_float] * 4 + [c_void_p] * 4),
+    "aa_categorical_workspace_bytes": (c_int64, [POINTER(CategoricalDesc)]),
+    "aa_categorical_log_prob": (c_int, [POINTER(CategoricalDesc), c_void_p, c_int64, c_void_p]),
+    "aa_categorical_log_prob_backward": (c_int, [POINTER(CategoricalDesc), c_void_p, c_void_p,
+                                                 c_void_p, c_int64, c_int64, c_void_p]),
+    "aa_clip_tensors_workspace_bytes": (c_int64, [POINTER(c_int64), c_int32]),
+    "aa_clip_tensors": (c_int, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64), c_int32,
+                                c_int32, c_double, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
+    "aa_layer_norm_forward": (c_int, [POINTER(LayerNormDesc), c_void_p]),
+    "aa_layer_norm_backward_workspace_bytes": (c_int64, [POINTER(LayerNormDesc)]),
+    "aa_layer_norm_backward": (c_int, [POINTER(LayerNormDesc), c_void_p, c_int64, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,624 @@
+// Log-probabilities of given actions (tokens) of Categorical(logits / temperature), with the entropy
+// and the most likely alternatives, and the gradient with respect to the logits.
+//   x = logits, -inf where the mask excludes an action;  c = 1 / temperature;  m: a reference of the row
+//   S = sum exp(c (x - m));   ln p_v = c (x_v - m) - ln S;   H = ln S - c sum exp(c (x - m)) (x - m) / S
+//   d x_v = c [ g (1{v = a} - p_v) - h p_v (ln p_v + H) ]        (g = d log_prob, h = d entropy)
+// One pass over a row: every lane keeps a reference r, S and sum e (x - r) relative to it, and moves r
+// only when a chunk exceeds it by CAT_MARGIN powers of two (exp never overflows, the sums lose nothing:
+// they are floating point); the lanes' triples are joined at the end.  Entropy is formed from
+// differences to the reference, never from two large numbers.  All sums are fp32.
+// The alternatives ride in the same pass: a wave keeps its 64 best keys (value, then lower index)
+// sorted across its lanes, a chunk whose maximum stays below the k-th costs one comparison, the others
+// collect in LDS and are merged 64 at a time by a bitonic network.
+// Bound by HBM for vocabularies, by launch and latency for a few actions.  Few rows: a row is split
+// over workgroups and the parts joined by a second launch.
+#include <math.h>
+#include "common.h"
+#include "agents_amd.h"
+#include "vec_types.h"
+
+#define CAT_MARGIN 4.f             // powers of two a value may exceed its lane's reference by
+#define CAT_LOWEST (-3.402823466e+38f)
+#define CAT_LOG2E 1.4426950408889634f
+#define CAT_LN2 0.6931471805599453f
+#define CAT_WAVE_VOCAB 4096        // up to here a wave takes a row, beyond a workgroup
+#define CAT_SPLIT_BLOCKS 1024      // workgroups that fill the machine
+#define CAT_EMPTY_KEY 0x007fffffffffffffull   // key of -inf: no alternative
+
+typedef unsigned long long u64;
+
+struct CatArgs {
+  int64_t rows, inner;
+  int vocab;
+  const void* logits; int64_t x_outer, x_inner;
+  const void* actions; int64_t a_outer, a_inner, first_action;
+  int action_bytes;
+  const void* mask; int64_t k_outer, k_inner;
+  float inv_t;                     // 1 / temperature
+  int top_k;
+  float* log_prob;
+  float* entropy;
+  float* stats;                    // [rows][2]: reference, ln S ((0, +inf) for a row without a distribution)
+  int64_t* top_ids;
+  float* top_log_prob;
+  int splits;                      // parts of a row
+  float* part;                     // [rows][splits][4]
+  u64* part_keys;                  // [rows][splits][top_k]
+};
+
+struct CatSum {
+  float r, s, t;
+};
+
+__device__ static inline float cat_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// moves `a` to the reference `to` (at or above a.r); a part whose weight vanishes leaves no trace
+// (its t may be infinite there), a NaN stays in s
+__device__ static inline CatSum cat_move(CatSum a, float to, float c2) {
+  const float d = fmaxf(a.r - to, CAT_LOWEST);
+  const float w = cat_exp2((a.r - to) * c2);
+  CatSum o;
+  o.r = to;
+  o.s = a.r == to ? a.s : a.s * w;
+  o.t = a.r == to ? a.t : w > 0.f ? w * (a.t + d * a.s) : 0.f;
+  return o;
+}
+
+__device__ static inline CatSum cat_join(CatSum a, CatSum b, float c2) {
+  const float to = fmaxf(a.r, b.r);
+  a = cat_move(a, to, c2);
+  b = cat_move(b, to, c2);
+  a.s += b.s;
+  a.t += b.t;
+  return a;
+}
+
+__device__ static inline CatSum cat_shfl_xor(CatSum a, int m) {
+  CatSum o;
+  o.r = __shfl_xor(a.r, m, 64);
+  o.s = __shfl_xor(a.s, m, 64);
+  o.t = __shfl_xor(a.t, m, 64);
+  return o;
+}
+
+// ---- alternatives: keys that order as (value, then lower index) ---------------------------------
+__device__ static inline u64 cat_key(float v, int index) {
+  const unsigned b = __float_as_uint(v + 0.f);             // -0 counts as 0
+  const unsigned hi = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return ((u64)hi << 32) | (unsigned)~index;
+}
+__device__ static inline float cat_key_value(u64 k) {
+  const unsigned hi = (unsigned)(k >> 32);
+  return __uint_as_float((hi & 0x80000000u) ? (hi & 0x7fffffffu) : ~hi);
+}
+__device__ static inline int cat_key_index(u64 k) { return (int)~(unsigned)k; }
+
+__device__ static inline u64 cat_sort_desc(u64 v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const u64 o = __shfl_xor(v, j, 64);
+      const bool larger = ((lane & j) == 0) == ((lane & k) == 0);
+      v = (larger == (v > o)) ? v : o;
+    }
+  return v;
+}
+
+// the 64 best of two descending lists
+__device__ static inline u64 cat_merge_desc(u64 a, u64 b, int lane) {
+  const u64 r = __shfl(b, 63 - lane, 64);
+  u64 v = a > r ? a : r;
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) {
+    const u64 o = __shfl_xor(v, j, 64);
+    v = (((lane & j) == 0) == (v > o)) ? v : o;
+  }
+  return v;
+}
+
+struct CatTop {
+  u64 list;          // this lane's place of the wave's best 64
+  u64 bar;           // a key must exceed it (wave-uniform)
+  int held;          // keys waiting in `buf` (wave-uniform)
+  u64* buf;          // 128 keys of LDS, this wave's own
+};
+
+__device__ static inline void cat_wave_fence() {
+  // LDS of one wave: executed in order, the compiler must keep it so
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ static inline void cat_top_merge(CatTop& t, u64 cand, int lane, int k) {
+  t.list = cat_merge_desc(t.list, cat_sort_desc(cand, lane), lane);
+  const u64 kth = __shfl(t.list, k - 1, 64);
+  if (kth > t.bar) t.bar = kth;
+}
+
+__device__ static inline void cat_top_flush(CatTop& t, int lane, int k) {
+  // the newest up to 64 waiting keys
+  const int n = t.held < 64 ? t.held : 64;
+  cat_wave_fence();
+  const u64 cand = lane < n ? t.buf[t.held - n + lane] : 0ull;
+  t.held -= n;
+  cat_wave_fence();
+  cat_top_merge(t, cand, lane, k);
+}
+
+__device__ static inline void cat_top_offer(CatTop& t, float v, int index, bool real, int lane,
+                                            int k) {
+  const u64 key = cat_key(v, index);
+  const bool in = real && key > t.bar;
+  const u64 b = __ballot(in);
+  if (b == 0ull) return;
+  if (in) t.buf[t.held + __popcll(b & ((1ull << lane) - 1ull))] = key;
+  t.held += __popcll(b);
+  if (t.held >= 64) cat_top_flush(t, lane, k);
+}
+
+// ---- the row's end: log_prob, entropy, stats, alternatives -----------------------------------------
+template <typename T, int MB>
+__device__ static inline bool cat_allowed(const CatArgs& a, int64_t row, int64_t v) {
+  if (MB == 0) return true;
+  const int64_t at = vt_row(row, a.inner, a.k_outer, a.k_inner) + v;
+  return MB == 1 ? reinterpret_cast<const uint8_t*>(a.mask)[at] != 0
+                 : reinterpret_cast<const int32_t*>(a.mask)[at] != 0;
+}
+
+__device__ static inline int64_t cat_action(const CatArgs& a, int64_t row) {
+  if (a.actions == nullptr) return 0;
+  const int64_t at = vt_row(row, a.inner, a.a_outer, a.a_inner);
+  const int64_t v = a.action_bytes == 8 ? reinterpret_cast<const int64_t*>(a.actions)[at]
+                                        : (int64_t)reinterpret_cast<const int32_t*>(a.actions)[at];
+  return v - a.first_action;
+}
+
+__device__ static inline float cat_nan() { return __uint_as_float(0x7fc00000u); }
+
+// one lane: everything of a row but its alternatives; returns ln S (+inf: no distribution)
+template <typename T, int MB>
+__device__ static inline float cat_finish(const CatArgs& a, int64_t row, int64_t action, CatSum u) {
+  const bool empty = u.s == 0.f;
+  const float ls = empty ? INFINITY : logf(u.s);
+  if (a.stats != nullptr) {
+    a.stats[2 * row] = empty ? 0.f : u.r;
+    a.stats[2 * row + 1] = ls;
+  }
+  if (a.entropy != nullptr) a.entropy[row] = empty ? 0.f : ls - a.inv_t * (u.t / u.s);
+  if (a.log_prob != nullptr) {
+    float lp;
+    if (action >= a.vocab) {
+      lp = cat_nan();
+    } else if (empty || !cat_allowed<T, MB>(a, row, action)) {
+      lp = isnan(ls) ? ls : -INFINITY;
+    } else {
+      const float x = T::one(reinterpret_cast<const typename T::elem*>(
+          a.logits)[vt_row(row, a.inner, a.x_outer, a.x_inner) + action]);
+      lp = (x - u.r) * a.inv_t - ls;
+    }
+    a.log_prob[row] = lp;
+  }
+  return ls;
+}
+
+// one wave: the row's alternatives from the sorted list
+__device__ static inline void cat_write_top(const CatArgs& a, int64_t row, int lane, u64 key, float r,
+                                            float ls) {
+  if (lane >= a.top_k) return;
+  const bool real = key > CAT_EMPTY_KEY && !isnan(ls);
+  a.top_ids[row * a.top_k + lane] = real ? cat_key_index(key) : -1;
+  a.top_log_prob[row * a.top_k + lane] =
+      real ? (cat_key_value(key) - r) * a.inv_t - ls : isnan(ls) ? ls : -INFINITY;
+}
+
+// a padding row (negative action): nothing of it is read
+__device__ static inline void cat_pad_row(const CatArgs& a, int64_t row, int lane) {
+  if (lane == 0) {
+    a.log_prob[row] = 0.f;
+    if (a.entropy != nullptr) a.entropy[row] = 0.f;
+    if (a.stats != nullptr) {
+      a.stats[2 * row] = 0.f;
+      a.stats[2 * row + 1] = INFINITY;
+    }
+  }
+  if (lane < a.top_k) {
+    a.top_ids[row * a.top_k + lane] = -1;
+    a.top_log_prob[row * a.top_k + lane] = -INFINITY;
+  }
+}
+
+// TEAM = 64: a wave per row, four rows per workgroup.  TEAM = 256: a workgroup per part of a row.
+template <typename T, int MB, int TEAM, bool TOP>
+__global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
+  constexpr int C = T::C;
+  __shared__ float red[3][4];
+  __shared__ u64 keys[TOP ? 4 : 1][TOP ? 128 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int me = TEAM == 64 ? lane : threadIdx.x;
+  const int64_t item = TEAM == 64 ? vt_block() * 4 + wave : vt_block();
+  const int64_t row = TEAM == 64 ? item : item / a.splits;
+  const int part = TEAM == 64 ? 0 : (int)(item - row * a.splits);
+  if (row >= a.rows) return;       // (the whole workgroup, or a wave that meets no barrier)
+  const int64_t action = cat_action(a, row);
+  if (action < 0) {
+    if (a.splits == 1) cat_pad_row(a, row, me);
+    return;                                     // the whole team returns; the joining launch writes
+  }
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
+                              vt_row(row, a.inner, a.x_outer, a.x_inner);
+  const uint8_t* mk = MB == 0 ? nullptr : reinterpret_cast<const uint8_t*>(a.mask) +
+                                              MB * vt_row(row, a.inner, a.k_outer, a.k_inner);
+  // chunks lie on 16-byte addresses: chunk k holds elements k C - skew ..
+  const int skew = (int)(((uintptr_t)x & 15u) / sizeof(typename T::elem));
+  const int chunks = (int)(((int64_t)a.vocab + skew + C - 1) / C);
+  const int each = TEAM == 64 ? chunks : (chunks + a.splits - 1) / a.splits;
+  const int k0 = part * each;
+  const int k1 = k0 + each < chunks ? k0 + each : chunks;
+  const float c2 = a.inv_t * CAT_LOG2E;
+  const float margin = CAT_MARGIN / c2;
+  CatSum u = {CAT_LOWEST, 0.f, 0.f};
+  CatTop top = {0ull, CAT_EMPTY_KEY, 0, TOP ? keys[wave] : nullptr};
+  for (int kb = k0 + (TEAM == 64 ? 0 : wave * 64); kb < k1; kb += TEAM) {   // (wave-uniform)
+    const int k = kb + lane;
+    const int e0 = k * C - skew;
+    float v[C];
+    if (k < k1 && e0 >= 0 && e0 + C <= a.vocab) {
+      T::widen(vt_load16(x + e0), v);
+      if (MB == 1) {
+        u64 m;
+        if (C == 8) {
+          __builtin_memcpy(&m, mk + e0, 8);
+        } else {
+          unsigned m4;
+          __builtin_memcpy(&m4, mk + e0, 4);
+          m = m4;
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (((m >> (8 * j)) & 0xffull) == 0ull) v[j] = -INFINITY;
+      }
+      if (MB == 4) {
+#pragma unroll
+        for (int j = 0; j < C; j += 4) {
+          const uint4 m = vt_load16(mk + 4 * (int64_t)(e0 + j));
+          if (m.x == 0u) v[j] = -INFINITY;
+          if (m.y == 0u) v[j + 1] = -INFINITY;
+          if (m.z == 0u) v[j + 2] = -INFINITY;
+          if (m.w == 0u) v[j + 3] = -INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int e = e0 + j;
+        v[j] = -INFINITY;
+        if (k < k1 && e >= 0 && e < a.vocab) {
+          v[j] = T::one(x[e]);
+          if (MB == 1 && mk[e] == 0) v[j] = -INFINITY;
+          if (MB == 4 && reinterpret_cast<const int32_t*>(mk)[e] == 0) v[j] = -INFINITY;
+        }
+      }
+    }
+    float high = v[0];
+#pragma unroll
+    for (int j = 1; j < C; ++j) high = fmaxf(high, v[j]);
+    if (high > u.r + margin) u = cat_move(u, high, c2);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const float d = v[j] - u.r;
+      const float e = cat_exp2(d * c2);
+      u.s += e;
+      u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
+    }
+    if (TOP) {
+      if (kb == k0 + (TEAM == 64 ? 0 : wave * 64)) {
+        // first round: k lanes have a chunk maximum at or above the k-th of the maxima, so the row's
+        // k best are too
+        const u64 kth = __shfl(cat_sort_desc(cat_key(high, 0), lane), a.top_k - 1, 64);
+        const u64 bar = kth & 0xffffffff00000000ull;
+        if (bar > top.bar) top.bar = bar;
+      }
+      if (__any(cat_key(high, 0) > top.bar)) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          cat_top_offer(top, v[j], e0 + j, k < k1 && v[j] > -INFINITY, lane, a.top_k);
+      }
+    }
+  }
+  if (TOP)
+    while (top.held > 0) cat_top_flush(top, lane, a.top_k);
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) u = cat_join(u, cat_shfl_xor(u, m), c2);
+  if constexpr (TEAM == 64) {
+    float ls = 0.f;
+    if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+    if (TOP) cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
+  } else {
+    if (lane == 0) { red[0][wave] = u.r; red[1][wave] = u.s; red[2][wave] = u.t; }
+    if (TOP) keys[wave][lane] = top.list;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      CatSum o = {red[0][w], red[1][w], red[2][w]};
+      u = cat_join(u, o, c2);
+      if (TOP) top.list = cat_merge_desc(top.list, keys[w][lane], lane);
+    }
+    if (a.splits == 1) {
+      float ls = 0.f;
+      if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+      if (TOP) cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
+    } else {
+      if (lane == 0) {
+        float* p = a.part + item * 4;
+        p[0] = u.r; p[1] = u.s; p[2] = u.t; p[3] = 0.f;
+      }
+      if (TOP && lane < a.top_k) a.part_keys[item * a.top_k + lane] = top.list;
+    }
+  }
+}
+
+// joins the parts of a row: a wave per row
+template <typename T, int MB, bool TOP>
+__global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
+  const int lane = threadIdx.x;
+  const int64_t row = vt_block();
+  if (row >= a.rows) return;
+  const int64_t action = cat_action(a, row);
+  if (action < 0) {
+    cat_pad_row(a, row, lane);
+    return;
+  }
+  const float c2 = a.inv_t * CAT_LOG2E;
+  CatSum u = {CAT_LOWEST, 0.f, 0.f};
+  for (int p = lane; p < a.splits; p += 64) {
+    const float* q = a.part + (row * a.splits + p) * 4;
+    CatSum o = {q[0], q[1], q[2]};
+    u = cat_join(u, o, c2);
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) u = cat_join(u, cat_shfl_xor(u, m), c2);
+  float ls = 0.f;
+  if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+  if (TOP) {
+    CatTop top = {0ull, CAT_EMPTY_KEY, 0, nullptr};
+    const int n = a.splits * a.top_k;
+    const u64* src = a.part_keys + row * n;
+    for (int i = 0; i < n; i += 64) {
+      const u64 key = i + lane < n ? src[i + lane] : 0ull;
+      if (__any(key > top.bar)) cat_top_merge(top, key, lane, a.top_k);
+    }
+    cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
+  }
+}
+
+// ---- gradient --------------------------------------------------------------------------------------
+struct CatGradArgs {
+  CatArgs f;                       // the forward's operands; stats and entropy as it left them
+  const float* dlog_prob;          // [rows], nullable
+  const float* dentropy;           // [rows], nullable
+  void* dx; int64_t dx_outer, dx_inner;
+  int blocks;                      // workgroups per row
+};
+
+struct CatRow {
+  float ref, c2, l2s, a0, a1, hit;
+  int action;
+  bool zero;
+};
+
+// d x_v = p_v (a0 + a1 (c2 (x - ref) - l2s)) + hit [v = action], p_v = 2^(c2 (x - ref) - l2s)
+__device__ static inline CatRow cat_row_grad(const CatGradArgs& a, int64_t row) {
+  CatRow o;
+  const int64_t action = cat_action(a.f, row);
+  const float ls = a.f.stats[2 * row + 1];
+  const float g = a.dlog_prob != nullptr ? a.dlog_prob[row] : 0.f;
+  const float h = a.dentropy != nullptr ? a.dentropy[row] : 0.f;
+  o.ref = a.f.stats[2 * row];
+  o.c2 = a.f.inv_t * CAT_LOG2E;
+  o.l2s = ls * CAT_LOG2E;
+  o.zero = action < 0 || (isinf(ls) && ls > 0.f);
+  const float ent = (a.dentropy != nullptr && !o.zero) ? a.f.entropy[row] : 0.f;
+  o.a0 = -a.f.inv_t * (g + h * ent);
+  o.a1 = -a.f.inv_t * h * CAT_LN2;
+  o.hit = a.f.inv_t * g;
+  // an action past the end: its log-probability is NaN, and so is the gradient
+  if (action >= a.f.vocab && a.dlog_prob != nullptr) o.a0 = cat_nan();
+  o.action = (a.dlog_prob != nullptr && action < a.f.vocab) ? (int)action : -1;
+  return o;
+}
+
+__device__ static inline float cat_grad_one(const CatRow& r, float x) {
+  const float l = fmaf(x - r.ref, r.c2, -r.l2s);
+  const float p = cat_exp2(l);
+  return p * fmaf(r.a1, fmaxf(l, -200.f), r.a0);       // (p is 0 from -150 on)
+}
+
+template <typename T, int MB>
+__global__ void __launch_bounds__(256) aa_categorical_grad_kernel(CatGradArgs a) {
+  constexpr int C = T::C;
+  const int64_t item = vt_block(), row = item / a.blocks;
+  const int block = (int)(item - row * a.blocks);
+  if (row >= a.f.rows) return;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.f.logits) +
+                              vt_row(row, a.f.inner, a.f.x_outer, a.f.x_inner);
+  typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.dx) +
+                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner);
+  const uint8_t* mk = MB == 0 ? nullptr : reinterpret_cast<const uint8_t*>(a.f.mask) +
+                                              MB * vt_row(row, a.f.inner, a.f.k_outer, a.f.k_inner);
+  const CatRow r = cat_row_grad(a, row);
+  // chunks lie on the destination's 16-byte addresses
+  const int skew = (int)(((uintptr_t)dx & 15u) / sizeof(typename T::elem));
+  const int chunks = (int)(((int64_t)a.f.vocab + skew + C - 1) / C);
+  for (int k = block * 256 + threadIdx.x; k < chunks; k += a.blocks * 256) {
+    const int e0 = k * C - skew;
+    if (e0 >= 0 && e0 + C <= a.f.vocab) {
+      float v[C];
+      T::widen(vt_load16(x + e0), v);
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = r.zero ? 0.f : cat_grad_one(r, v[j]);
+      if ((unsigned)(r.action - e0) < (unsigned)C && !r.zero) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (e0 + j == r.action) v[j] += r.hit;
+      }
+      if (MB == 1) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (mk[e0 + j] == 0) v[j] = 0.f;
+      }
+      if (MB == 4) {
+#pragma unroll
+        for (int j = 0; j < C; j += 4) {
+          const uint4 m = vt_load16(mk + 4 * (int64_t)(e0 + j));
+          if (m.x == 0u) v[j] = 0.f;
+          if (m.y == 0u) v[j + 1] = 0.f;
+          if (m.z == 0u) v[j + 2] = 0.f;
+          if (m.w == 0u) v[j + 3] = 0.f;
+        }
+      }
+      vt_store16(dx + e0, T::pack(v));
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int e = e0 + j;
+        if (e < 0 || e >= a.f.vocab) continue;
+        float v = r.zero ? 0.f : cat_grad_one(r, T::one(x[e]));
+        if (e == r.action && !r.zero) v += r.hit;
+        if (MB == 1 && mk[e] == 0) v = 0.f;
+        if (MB == 4 && reinterpret_cast<const int32_t*>(mk)[e] == 0) v = 0.f;
+        dx[e] = T::put(v);
+      }
+    }
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+static int cat_check(const aa_categorical_desc* d) {
+  if (d == nullptr || d->rows <= 0 || d->inner <= 0 || d->vocab <= 0 || d->logits == nullptr)
+    return AA_ERR_INVALID;
+  if (d->dtype < AA_DT_F32 || d->dtype > AA_DT_F16) return AA_ERR_INVALID;
+  if (d->actions != nullptr && d->action_bytes != 4 && d->action_bytes != 8) return AA_ERR_INVALID;
+  if (d->mask != nullptr && d->mask_bytes != 1 && d->mask_bytes != 4) return AA_ERR_INVALID;
+  if (!(d->temperature >= 1e-30f && d->temperature <= 1e30f)) return AA_ERR_INVALID;
+  if (d->top_k < 0 || d->top_k > AA_CATEGORICAL_MAX_TOP || d->top_k > d->vocab)
+    return AA_ERR_INVALID;
+  if (d->vocab > (1 << 30)) return AA_ERR_RANGE;
+  return AA_OK;
+}
+
+static int cat_splits(const aa_categorical_desc* d) {
+  if (d->vocab <= CAT_WAVE_VOCAB) return 1;
+  const int per = d->dtype == AA_DT_F32 ? 4 : 8;
+  int64_t want = (CAT_SPLIT_BLOCKS + d->rows - 1) / d->rows;
+  const int64_t most = (d->vocab / per + 1023) / 1024;     // four rounds of a workgroup at least
+  if (want > most) want = most;
+  return want < 1 ? 1 : (int)want;
+}
+
+static CatArgs cat_args(const aa_categorical_desc* d) {
+  CatArgs a;
+  a.rows = d->rows; a.inner = d->inner; a.vocab = (int)d->vocab;
+  a.logits = d->logits; a.x_outer = d->x_outer; a.x_inner = d->x_inner;
+  a.actions = d->actions; a.a_outer = d->a_outer; a.a_inner = d->a_inner;
+  a.first_action = d->first_action; a.action_bytes = d->action_bytes;
+  a.mask = d->mask; a.k_outer = d->k_outer; a.k_inner = d->k_inner;
+  a.inv_t = 1.f / d->temperature; a.top_k = d->top_k;
+  a.log_prob = d->log_prob; a.entropy = d->entropy; a.stats = d->stats;
+  a.top_ids = d->top_ids; a.top_log_prob = d->top_log_prob;
+  a.splits = 1; a.part = nullptr; a.part_keys = nullptr;
+  return a;
+}
+
+template <typename T, int MB>
+static void cat_launch(const CatArgs& a, hipStream_t st) {
+  if (a.vocab <= CAT_WAVE_VOCAB) {
+    const dim3 grid = vt_grid((a.rows + 3) / 4);
+    if (a.top_k > 0) aa_categorical_kernel<T, MB, 64, true><<<grid, dim3(256), 0, st>>>(a);
+    else aa_categorical_kernel<T, MB, 64, false><<<grid, dim3(256), 0, st>>>(a);
+    return;
+  }
+  const dim3 grid = vt_grid(a.rows * a.splits);
+  if (a.top_k > 0) aa_categorical_kernel<T, MB, 256, true><<<grid, dim3(256), 0, st>>>(a);
+  else aa_categorical_kernel<T, MB, 256, false><<<grid, dim3(256), 0, st>>>(a);
+  if (a.splits > 1) {
+    const dim3 rows = vt_grid(a.rows);
+    if (a.top_k > 0) aa_categorical_join_kernel<T, MB, true><<<rows, dim3(64), 0, st>>>(a);
+    else aa_categorical_join_kernel<T, MB, false><<<rows, dim3(64), 0, st>>>(a);
+  }
+}
+
+template <typename T>
+static void cat_launch_grad(const CatGradArgs& g, int mask_bytes, hipStream_t st) {
+  const dim3 grid = vt_grid(g.f.rows * g.blocks);
+  if (mask_bytes == 0) aa_categorical_grad_kernel<T, 0><<<grid, dim3(256), 0, st>>>(g);
+  else if (mask_bytes == 1) aa_categorical_grad_kernel<T, 1><<<grid, dim3(256), 0, st>>>(g);
+  else aa_categorical_grad_kernel<T, 4><<<grid, dim3(256), 0, st>>>(g);
+}
+
+template <typename T>
+static void cat_launch_mask(const CatArgs& a, int mask_bytes, hipStream_t st) {
+  if (mask_bytes == 0) cat_launch<T, 0>(a, st);
+  else if (mask_bytes == 1) cat_launch<T, 1>(a, st);
+  else cat_launch<T, 4>(a, st);
+}
+
+extern "C" {
+
+int64_t aa_categorical_workspace_bytes(const aa_categorical_desc* d) {
+  if (cat_check(d) != AA_OK) return -1;
+  const int splits = cat_splits(d);
+  return splits == 1 ? 0 : d->rows * splits * (16 + 8 * (int64_t)d->top_k);
+}
+
+int aa_categorical_log_prob(const aa_categorical_desc* d, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  const int rc = cat_check(d);
+  if (rc != AA_OK) return rc;
+  if ((d->actions == nullptr) != (d->log_prob == nullptr)) return AA_ERR_INVALID;
+  if (d->top_k > 0 && (d->top_ids == nullptr || d->top_log_prob == nullptr)) return AA_ERR_INVALID;
+  const int64_t need = aa_categorical_workspace_bytes(d);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return AA_ERR_RANGE;
+  CatArgs a = cat_args(d);
+  a.splits = cat_splits(d);
+  if (a.rows * a.splits > VT_MAX_BLOCKS) return AA_ERR_RANGE;
+  if (a.splits > 1) {
+    a.part = (float*)workspace;
+    a.part_keys = (u64*)(a.part + 4 * a.rows * a.splits);
+  }
+  const int mb = d->mask == nullptr ? 0 : d->mask_bytes;
+  hipStream_t st = (hipStream_t)stream;
+  if (d->dtype == AA_DT_F32) cat_launch_mask<VtF32>(a, mb, st);
+  else if (d->dtype == AA_DT_BF16) cat_launch_mask<VtBf16>(a, mb, st);
+  else cat_launch_mask<VtF16>(a, mb, st);
+  return aa_launch_status();
+}
+
+int aa_categorical_log_prob_backward(const aa_categorical_desc* d, const float* dlog_prob,
+                                     const float* dentropy, void* dlogits, int64_t dx_outer,
+                                     int64_t dx_inner, void* stream) {
+  const int rc = cat_check(d);
+  if (rc != AA_OK) return rc;
+  if (d->stats == nullptr || dlogits == nullptr || (dlog_prob == nullptr && dentropy == nullptr) ||
+      (dlog_prob != nullptr && d->actions == nullptr) ||
+      (dentropy != nullptr && d->entropy == nullptr))
+    return AA_ERR_INVALID;
+  CatGradArgs g;
+  g.f = cat_args(d);
+  g.dlog_prob = dlog_prob; g.dentropy = dentropy;
+  g.dx = dlogits; g.dx_outer = dx_outer; g.dx_inner = dx_inner;
+  const int per = d->dtype == AA_DT_F32 ? 4 : 8;
+  const int64_t rounds = (d->vocab / per + 256) / 256;
+  g.blocks = (int)((rounds + 3) / 4);
+  if (g.f.rows * g.blocks > VT_MAX_BLOCKS) return AA_ERR_RANGE;
+  const int mb = d->mask == nullptr ? 0 : d->mask_bytes;
+  hipStream_t st = (hipStream_t)stream;
+  if (d->dtype == AA_DT_F32) cat_launch_grad<VtF32>(g, mb, st);
+  else if (d->dtype == AA_DT_BF16) cat_launch_grad<VtBf16>(g, mb, st);
+  else cat_launch_grad<VtF16>(g, mb, st);
+  return aa_launch_status();
+}
+
+}  // extern "C"

@@ -1066,6 +1066,92 @@ int aa_norm_apply(const float* x, int64_t n_outer, int64_t n_inner, const float*
                   const float* var_num, const float* var_den, float variance_epsilon,
                   float clip_value, float* out, void* stream);
 
+/* =========================================================================================
+ * Operators of policies over many discrete actions (tokens)
+ *   Rows of float32 / bfloat16 / float16 (`dtype`: AA_DT_*).  A [.., n] tensor whose leading axes
+ *   fold to (rows / inner, inner) is described by two strides in elements: row r starts at
+ *   (r / inner) * outer + (r % inner) * inner_stride; the last axis is contiguous.  Sums, statistics
+ *   and weights are float32.
+ * ========================================================================================= */
+#define AA_DT_F32 0
+#define AA_DT_BF16 1
+#define AA_DT_F16 2
+
+/* Categorical(logits / temperature): log-probabilities of given actions, entropy, most likely
+ * alternatives (tfp Categorical.log_prob / entropy as policies use them; csrc/categorical.hip).
+ *   mask [rows, vocab] (nullable; bytes or int32, 0 excludes an action: probability 0 exactly).
+ *   action index = actions[r] - first_action.  Negative: a padding row -- log_prob, entropy and
+ *   gradient are 0, its logits are not used.  Past the end: log_prob and gradient are NaN.
+ *   A row without any allowed finite logit: log_prob -inf, entropy 0, gradient 0.  NaN or +inf in an
+ *   allowed place: NaN.
+ *   top_k <= AA_CATEGORICAL_MAX_TOP (and <= vocab): ids (without first_action) and log-probabilities
+ *   by descending logit, equal ones by ascending index; -1 / -inf where fewer have a probability.
+ *   stats [rows][2] is what the backward call needs besides `entropy`. */
+#define AA_CATEGORICAL_MAX_TOP 64
+typedef struct aa_categorical_desc {
+  int64_t rows, inner, vocab;
+  const void* logits;
+  int64_t x_outer, x_inner;
+  const void* actions;          /* nullable together with log_prob */
+  int64_t a_outer, a_inner, first_action;
+  const void* mask;             /* nullable */
+  int64_t k_outer, k_inner;
+  int32_t dtype, action_bytes /* 4 or 8 */, mask_bytes /* 1 or 4 */, top_k;
+  float temperature;            /* 1e-30 .. 1e30 */
+  float* log_prob;              /* [rows] */
+  float* entropy;               /* [rows], nullable */
+  float* stats;                 /* [rows][2], nullable in the forward call */
+  int64_t* top_ids;             /* [rows][top_k] */
+  float* top_log_prob;          /* [rows][top_k] */
+} aa_categorical_desc;
+int64_t aa_categorical_workspace_bytes(const aa_categorical_desc* d);
+int aa_categorical_log_prob(const aa_categorical_desc* d, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+/* dlogits[r][v] = d loss / d logits from d loss / d log_prob and d loss / d entropy (either nullable);
+ * written in the logits' type for every v, may be the logits' own storage if the layout is the same. */
+int aa_categorical_log_prob_backward(const aa_categorical_desc* d, const float* dlog_prob,
+                                     const float* dentropy, void* dlogits, int64_t dx_outer,
+                                     int64_t dx_inner, void* stream);
+
+/* tf.clip_by_global_norm (each = 0) / tf.clip_by_norm per tensor (each = 1) over n_tensors tensors of
+ * their own contiguous storage and one type (ppo_agent.py:948-949, eager_utils.py:227-246;
+ * csrc/grad_clip.hip).  dst_h[i] may be src_h[i].  norm: [1] or [n_tensors] float32.  A norm that is
+ * not finite makes the values it scales NaN.  dst_h NULL (each = 0): the norm only. */
+#define AA_CLIP_TENSORS 96      /* tensors per launch */
+int64_t aa_clip_tensors_workspace_bytes(const int64_t* n_h, int32_t n_tensors);
+int aa_clip_tensors(const void* const* src_h, void* const* dst_h, const int64_t* n_h,
+                    int32_t n_tensors, int32_t dtype, double clip, int32_t each, float* norm,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* keras LayerNormalization over the last axis (csrc/layer_norm.hip):
+ *   y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(mean((x - mean)^2) + epsilon)
+ * gamma / beta [width] float32, nullable (1 / 0).  stats [rows][2] receives mean, rstd (nullable in
+ * the forward call).  Backward: dx (nullable) is multiplied by act'(x) for mask_act != AA_ACT_NONE,
+ * x being the output of that activation; dgamma / dbeta (each nullable) are overwritten.  y may be x,
+ * dx may be x or dy. */
+typedef struct aa_layer_norm_desc {
+  int64_t rows, inner, width;
+  const void* x;
+  int64_t x_outer, x_inner;
+  const void* dy;
+  int64_t dy_outer, dy_inner;
+  void* y;
+  int64_t y_outer, y_inner;
+  void* dx;
+  int64_t dx_outer, dx_inner;
+  const float* gamma;
+  const float* beta;
+  float* stats;
+  float* dgamma;
+  float* dbeta;
+  float epsilon;
+  int32_t dtype, mask_act;
+} aa_layer_norm_desc;
+int aa_layer_norm_forward(const aa_layer_norm_desc* d, void* stream);
+int64_t aa_layer_norm_backward_workspace_bytes(const aa_layer_norm_desc* d);
+int aa_layer_norm_backward(const aa_layer_norm_desc* d, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

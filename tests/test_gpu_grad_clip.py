@@ -1,0 +1,149 @@
+"""clip_by_global_norm / clip_by_norms / global_norm against the float64 statement (oracle/grad_clip.py).
+
+Tolerances: the norm is summed in float64 and rounded once (u = 2^-24); a clipped value carries the
+factor's rounding and the product's (2 u) and half a step of its type.
+"""
+import numpy as np
+import pytest
+import torch
+
+from agents_amd import ops
+from oracle import grad_clip as oclip
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def f64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def check(ts, clip, each, got, norm):
+    want, wn = (oclip.clip_by_norms if each else oclip.clip_by_global_norm)([f64(t) for t in ts], clip)
+    n = f64(norm)
+    bad = ~np.isfinite(wn)
+    np.testing.assert_array_equal(np.isnan(np.atleast_1d(n)[np.atleast_1d(bad)]),
+                                  np.isnan(np.atleast_1d(wn)[np.atleast_1d(bad)]))
+    with np.errstate(invalid="ignore"):
+        assert np.all(bad | (np.abs(n - wn) <= 2 * U * np.abs(wn) + 2.0 ** -149))
+    half = torch.finfo(ts[0].dtype).eps / 2
+    tiny = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[
+        ts[0].dtype]
+    for t, w, g in zip(ts, want, got):
+        assert g.dtype == t.dtype and g.shape == t.shape
+        d = f64(g)
+        nan = np.isnan(w)
+        np.testing.assert_array_equal(np.isnan(d), nan)
+        assert np.all(nan | (np.abs(d - w) <= (3 * U + half * (1 + 3 * U)) * np.abs(w) + tiny / 2))
+
+
+def grads(sizes, dtype, dev, seed=0, scale=0.1):
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    return [(torch.randn(s, generator=gen, device=dev) * scale).to(dtype) for s in sizes]
+
+
+SETS = {"one": [(1,)], "scalars": [(), (), (3,)], "odd": [(7,), (8193,), (3, 5, 11), (1,)],
+        "empty": [(0,), (5,), (0, 4), (100,)], "pieces": [(8192,), (8193,), (16385,), (300001,)],
+        "hundred": [(i + 1,) for i in range(100)], "many": [(17 + i % 50,) for i in range(500)]}
+
+
+@pytest.mark.parametrize("sizes", list(SETS))
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("clip", [0.05, 1e6])
+def test_clip(dev, sizes, dtype, clip):
+    ts = grads(SETS[sizes], dtype, dev)
+    got, norm = ops.clip_by_global_norm(ts, clip)
+    assert norm.shape == ()
+    check(ts, clip, False, got, norm)
+    got, norms = ops.clip_by_norms(ts, clip)
+    assert norms.shape == (len(ts),)
+    check(ts, clip, True, got, norms)
+    assert torch.equal(ops.global_norm(ts), ops.clip_by_global_norm(ts, clip)[1])
+
+
+def test_more_pieces_than_one_workgroup_joins(dev):
+    ts = grads([(2,)] * 5000, torch.float32, dev)
+    got, norm = ops.clip_by_global_norm(ts, 0.5)
+    check(ts, 0.5, False, got, norm)
+    assert torch.equal(norm, ops.global_norm(ts))
+
+
+def test_large_and_unaligned(dev):
+    gen = torch.Generator(device=dev).manual_seed(3)
+    flat = torch.randn(30_000_011, generator=gen, device=dev) * 0.01
+    for dtype in TYPES:
+        f = flat.to(dtype)
+        ts = [f[1:5_000_000], f[5_000_003:29_000_000], f[29_000_001:]]
+        check(ts, 2.0, False, *ops.clip_by_global_norm(ts, 2.0))
+        out = torch.full_like(f, 3.0)
+        outs = [out[3:5_000_002], out[5_000_005:29_000_002], out[29_000_010:-9 + len(out)]]
+        outs[2] = out[29_000_010:29_000_010 + 1_000]
+        ts[2] = ts[2][:1000]
+        got, _ = ops.clip_by_global_norm(ts, 2.0, out=outs)
+        for g, w in zip(outs, ops.clip_by_global_norm(ts, 2.0)[0]):
+            assert torch.equal(g, w)
+        assert (out[:3] == 3).all() and (out[5_000_002:5_000_005] == 3).all() and \
+            (out[29_000_002:29_000_010] == 3).all() and (out[29_001_010:] == 3).all()
+
+
+def test_in_place(dev):
+    ts = grads(SETS["odd"], torch.float32, dev, 5)
+    want, norm = ops.clip_by_global_norm(ts, 0.3)
+    got, n2 = ops.clip_by_global_norm(ts, 0.3, out=ts)
+    assert torch.equal(norm, n2) and all(a is b for a, b in zip(got, ts))
+    for a, b in zip(ts, want):
+        assert torch.equal(a, b)
+
+
+def test_unclipped_values_are_the_same_bits(dev):
+    ts = grads(SETS["odd"], torch.bfloat16, dev, 6)
+    got, norm = ops.clip_by_global_norm(ts, 1e4)
+    assert all(torch.equal(a, b) for a, b in zip(got, ts))
+
+
+@pytest.mark.parametrize("value", [1e30, 1e-30])
+def test_squares_outside_float32(dev, value):
+    ts = [torch.full((1000,), value, device=dev), torch.full((24,), value, device=dev)]
+    check(ts, value, False, *ops.clip_by_global_norm(ts, value))
+    check(ts, value, True, *ops.clip_by_norms(ts, value))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_not_finite(dev, bad):
+    ts = grads([(50,), (9000,), (3,)], torch.float32, dev, 7)
+    ts[1][8999] = bad
+    got, norm = ops.clip_by_global_norm(ts, 0.1)
+    assert all(g.isnan().all() for g in got) and not torch.isfinite(norm)
+    got, norms = ops.clip_by_norms(ts, 0.1)
+    assert got[1].isnan().all() and not got[0].isnan().any() and not got[2].isnan().any()
+    check(ts, 0.1, True, got, norms)
+
+
+def test_same_bits_on_two_streams_and_in_a_graph(dev):
+    a = grads(SETS["pieces"], torch.float32, dev, 8)
+    b = grads(SETS["pieces"], torch.float32, dev, 9)
+    wa, wb = ops.clip_by_global_norm(a, 0.4), ops.clip_by_global_norm(b, 0.4)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            got.append((ops.clip_by_global_norm(a, 0.4), wa))
+        with torch.cuda.stream(s2):
+            got.append((ops.clip_by_global_norm(b, 0.4), wb))
+    torch.cuda.synchronize()
+    for (x, n), (y, m) in got:
+        assert torch.equal(n, m) and all(torch.equal(p, q) for p, q in zip(x, y))
+    live = [t.clone() for t in a]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, norm = ops.clip_by_global_norm(live, 0.4)
+    for i in range(6):
+        for t, s in zip(live, a if i % 2 == 0 else b):
+            t.copy_(s)
+        graph.replay()
+        e, n = ops.clip_by_global_norm(live, 0.4)
+        torch.cuda.synchronize()
+        assert torch.equal(n, norm) and all(torch.equal(p, q) for p, q in zip(out, e))

@@ -1,0 +1,240 @@
+"""layer_norm_forward / layer_norm_backward against the float64 statement (oracle/layer_norm.py).
+
+Tolerances (u = 2^-24): a row's sum has chains of at most D / team + 30 additions (`chain`), so the mean
+is off by chain u max|x|, the normalised value h by `he` = (chain max|x| rstd + (chain + 8) |h|) u (the
+variance's relative error halves under the root), y by he |gamma| + 3 u (|h gamma| + |beta|) and half a
+step of its type.  dx = rstd (g - c1 - h c2): c1 and c2 are means with chain u of their terms' size and
+he |g| of h's error.  The weights' sums run over rows: `rows_chain` additions.
+"""
+import numpy as np
+import pytest
+import torch
+
+from agents_amd import ops
+from oracle import layer_norm as oln
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def f64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def chain(d):
+    return max(16.0, d / 1024.0) + 34.0
+
+
+def tiny(dtype):
+    return {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}[dtype]
+
+
+def h_error(x, h, rstd):
+    c = chain(x.shape[-1])
+    return U * (c * np.abs(x).max(-1, keepdims=True) * rstd[..., None] + (c + 8) * np.abs(h))
+
+
+def check_forward(x, gamma, beta, eps, y, stats):
+    xd = f64(x)
+    g = None if gamma is None else f64(gamma)
+    b = None if beta is None else f64(beta)
+    want, mean, rstd = oln.forward(xd, g, b, eps)
+    h, _, _ = oln.forward(xd, None, None, eps)
+    he = h_error(xd, h, rstd)
+    gs = 1.0 if g is None else np.abs(g)
+    bs = 0.0 if b is None else np.abs(b)
+    half = torch.finfo(x.dtype).eps / 2
+    tol = (he * gs + 3 * U * (np.abs(h) * gs + bs)) * (1 + half) + half * np.abs(want) + tiny(x.dtype)
+    err = np.abs(f64(y) - want)
+    assert np.all(err <= tol), (err / tol).max()
+    c = chain(x.shape[-1])
+    assert np.all(np.abs(f64(stats)[..., 0] - mean) <= U * c * (np.abs(xd).max(-1) + 1e-30))
+    # var relative: 2 (chain) u, and the mean's error squared about itself
+    me = U * c * np.abs(xd).max(-1) * rstd
+    assert np.all(np.abs(f64(stats)[..., 1] / rstd - 1) <= U * (c + 8) + me * me)
+
+
+def act_grad(x, act):
+    return 1.0 if act is None else (x > 0) * 1.0 if act == "relu" else 1 - x * x
+
+
+def check_backward(dy, x, gamma, eps, out, act=None):
+    dx, dg, db = out
+    xd, dyd = f64(x), f64(dy)
+    g = None if gamma is None else f64(gamma)
+    wx, wg, wb = oln.backward(dyd, xd, g, eps)
+    h, _, rstd = oln.forward(xd, None, None, eps)
+    D = x.shape[-1]
+    he = h_error(xd, h, rstd)
+    if dx is not None:
+        gr = dyd if g is None else dyd * g
+        a = act_grad(xd, act)
+        c = chain(D)
+        m = lambda t: np.abs(t).mean(-1, keepdims=True)
+        c1 = U * (c + 2) * m(gr)
+        c2 = U * (c + 4) * m(gr * h) + m(gr * he)
+        tol = rstd[..., None] * (c1 + c2 * np.abs(h) + he * np.abs((gr * h).mean(-1, keepdims=True)) +
+                                 6 * U * (np.abs(gr) + m(gr) + np.abs(h) * m(gr * h)))
+        half = torch.finfo(x.dtype).eps / 2
+        # the saved 1 / sqrt(var + eps) is off by what check_forward allows
+        tol = tol + np.abs(wx) * U * (c + 8)
+        tol = tol * np.abs(a) * (1 + half) + 3 * U * np.abs(wx * a) + half * np.abs(wx * a) + \
+            tiny(x.dtype)
+        err = np.abs(f64(dx) - wx * a)
+        assert np.all(err <= tol), (err / tol).max()
+    if dg is not None:
+        rows = tuple(range(xd.ndim - 1))
+        n = int(np.prod(xd.shape[:-1]))
+        rc = n / 64.0 + 80
+        tol = U * rc * np.abs(dyd * h).sum(rows) + (np.abs(dyd) * he).sum(rows) + 1e-30
+        assert np.all(np.abs(f64(dg) - wg) <= tol), (np.abs(f64(dg) - wg) / tol).max()
+        tol = U * rc * np.abs(dyd).sum(rows) + 1e-30
+        assert np.all(np.abs(f64(db) - wb) <= tol), (np.abs(f64(db) - wb) / tol).max()
+
+
+def inputs(shape, dtype, dev, seed, mean=0.5):
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=gen, device=dev)
+    x = (n(*shape) * 1.5 + mean).to(dtype)
+    dy = n(*shape).to(dtype)
+    return x, dy, 1 + 0.3 * n(shape[-1]), 0.3 * n(shape[-1])
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 2), (5, 3), (3, 17), (257, 64), (2, 3, 255), (1, 512),
+                                   (1025, 100), (6, 1003), (4, 1024), (3, 1025), (5, 4096), (2, 4100),
+                                   (2, 8192), (3, 8201), (2, 16384), (3, 16385), (70, 20011), (1, 40000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_backward(dev, shape, dtype):
+    x, dy, gamma, beta = inputs(shape, dtype, dev, sum(shape))
+    y, stats = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    check_forward(x, gamma, beta, 1e-3, y, stats)
+    check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
+
+
+@pytest.mark.parametrize("shape", [(9, 130), (5, 5000), (3, 20000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_without_weights_masks_parts(dev, shape, dtype):
+    x, dy, gamma, beta = inputs(shape, dtype, dev, 3)
+    y, stats = ops.layer_norm_forward(x, None, None, 1e-5)
+    check_forward(x, None, None, 1e-5, y, stats)
+    y, stats = ops.layer_norm_forward(x, None, beta, 1e-5)
+    check_forward(x, None, beta, 1e-5, y, stats)
+    check_backward(dy, x, None, 1e-5, ops.layer_norm_backward(dy, x, None, stats))
+    out = ops.layer_norm_backward(dy, x, gamma, stats, param_grads=False)
+    assert out[1] is None and out[2] is None
+    check_backward(dy, x, gamma, 1e-5, out)
+    out = ops.layer_norm_backward(dy, x, gamma, stats, input_grad=False)
+    assert out[0] is None
+    check_backward(dy, x, gamma, 1e-5, out)
+    for act in ("relu", "tanh"):
+        xa = torch.relu(x) if act == "relu" else torch.tanh(x.float()).to(dtype)
+        _, st = ops.layer_norm_forward(xa, gamma, beta, 1e-5)
+        check_backward(dy, xa, gamma, 1e-5,
+                       ops.layer_norm_backward(dy, xa, gamma, st, mask_act=act), act)
+
+
+@pytest.mark.parametrize("mean", [0.0, 100.0, -3000.0])
+def test_rows_far_from_zero(dev, mean):
+    """The variance is taken about the mean: a common offset costs only the inputs' own rounding."""
+    x, dy, gamma, beta = inputs((7, 700), torch.float32, dev, 4, mean)
+    y, stats = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    check_forward(x, gamma, beta, 1e-3, y, stats)
+    check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
+
+
+def test_constant_rows_and_infinities(dev):
+    x = torch.full((4, 300), 2.0, device=dev)
+    gamma, beta = torch.ones(300, device=dev), torch.zeros(300, device=dev)
+    y, stats = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    assert (y == 0).all() and (stats[:, 0] == 2).all()
+    x[1, 7] = float("nan")
+    x[2, 9] = float("inf")
+    y, _ = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    assert (y[0] == 0).all() and (y[3] == 0).all()        # rows do not meet
+    assert y[1].isnan().all() and y[2].isnan().any()
+
+
+def test_strides_and_in_place(dev):
+    gen = torch.Generator(device=dev).manual_seed(6)
+    for D in (33, 2000, 17001):
+        wide = torch.randn(4, 5, D + 9, generator=gen, device=dev).half()
+        x = wide[:, 1:4, 3:3 + D]
+        dy = torch.randn(4, 1, D, generator=gen, device=dev).half().expand(4, 3, D)
+        gamma = torch.rand(D + 1, generator=gen, device=dev)[1:]
+        beta = torch.rand(D, generator=gen, device=dev)
+        y, stats = ops.layer_norm_forward(x, gamma, beta)
+        check_forward(x, gamma, beta, 1e-3, y, stats)
+        ref = ops.layer_norm_backward(dy, x, gamma, stats)
+        check_backward(dy, x, gamma, 1e-3, ref)
+        buf = torch.full((4, 3, D + 4), 5.0, dtype=torch.float16, device=dev)
+        out = buf[..., 1:1 + D]
+        ops.layer_norm_forward(x, gamma, beta, out=out)
+        assert torch.equal(out, y) and (buf[..., 0] == 5).all() and (buf[..., D + 1:] == 5).all()
+        xc = x.contiguous()
+        ops.layer_norm_forward(xc, gamma, beta, out=xc)
+        assert torch.equal(xc, y)
+        for alias in ("dy", "x"):
+            a, b = dy.contiguous(), x.contiguous()
+            got = ops.layer_norm_backward(a, b, gamma, stats, dx=a if alias == "dy" else b)
+            for p, q in zip(got, ref):
+                assert torch.equal(p, q)
+
+
+def test_no_rows(dev):
+    x = torch.empty(0, 5, device=dev)
+    y, stats = ops.layer_norm_forward(x, None, None)
+    dx, dg, db = ops.layer_norm_backward(x, x, None, stats)
+    assert y.shape == (0, 5) and dx.shape == (0, 5) and (dg == 0).all() and (db == 0).all()
+
+
+def test_many_rows_and_far_offsets(dev):
+    n = (1 << 22) + 7                       # more rows than one grid axis takes workgroups
+    x = torch.randn(n, 4, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    y, stats = ops.layer_norm_forward(x, None, None)
+    xd = x.double()
+    h = (xd - xd.mean(1, keepdim=True)) / (xd.var(1, unbiased=False, keepdim=True) + 1e-3).sqrt()
+    assert (y.double() - h).abs().max() < 1e-5      # |x| rstd <= 6 / sqrt(1e-3): chain u 190 = 6e-6
+    stride = (1 << 31) + 1001
+    buf = torch.empty(stride + 1001, dtype=torch.float16, device=dev)
+    x = buf.as_strided((2, 1001), (stride, 1))
+    x.copy_(torch.randn(2, 1001, generator=torch.Generator().manual_seed(2)))
+    y, stats = ops.layer_norm_forward(x, None, None)
+    check_forward(x, None, None, 1e-3, y, stats)
+    dy = torch.ones(2, 1001, dtype=torch.float16, device=dev)
+    check_backward(dy, x, None, 1e-3, ops.layer_norm_backward(dy, x, None, stats))
+
+
+def test_same_bits_on_two_streams_and_in_a_graph(dev):
+    x, dy, gamma, beta = inputs((600, 1500), torch.bfloat16, dev, 8)
+    x2, dy2, _, _ = inputs((600, 1500), torch.bfloat16, dev, 9)
+
+    def both(a, b):
+        y, st = ops.layer_norm_forward(a, gamma, beta)
+        return (y, st) + ops.layer_norm_backward(b, a, gamma, st)
+
+    w1, w2 = both(x, dy), both(x2, dy2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            got.append((both(x, dy), w1))
+        with torch.cuda.stream(s2):
+            got.append((both(x2, dy2), w2))
+    torch.cuda.synchronize()
+    for a, b in got:
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+    xs, ds = x.clone(), dy.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(xs, ds)
+    for i in range(6):
+        xs.copy_(x if i % 2 == 0 else x2)
+        graph.replay()
+        eager = both(xs, ds)
+        torch.cuda.synchronize()
+        for p, q in zip(out, eager):
+            assert torch.equal(p, q)
