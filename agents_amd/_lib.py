@@ -460,6 +460,33 @@ def load():
     return lib
 
 
+_bind = None
+
+
+def load_token_ops():
+    """Loads the CPython module in front of the token operators (csrc/token_ops_bind.cpp) once and
+    hands it the library's entries.  Raises if it has not been built."""
+    global _bind
+    if _bind is not None:
+        return _bind
+    lib = load()
+    try:
+        from agents_amd import _token_ops
+    except ImportError as e:
+        raise AgentsAmdError(f"agents_amd/_token_ops.so is missing or does not load ({e}): build it "
+                             "with `python -m agents_amd._build`") from e
+    entries = ("aa_categorical_workspace_bytes", "aa_categorical_log_prob",
+               "aa_categorical_log_prob_backward", "aa_clip_tensors_workspace_bytes",
+               "aa_clip_tensors", "aa_layer_norm_forward",
+               "aa_layer_norm_backward_workspace_bytes", "aa_layer_norm_backward")
+    raw = _RAW_STREAM if _RAW_STREAM is not None else \
+        (lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _token_ops.init(tuple(ctypes.cast(getattr(lib, n), c_void_p).value for n in entries), raw,
+                    AgentsAmdError)
+    _bind = _token_ops
+    return _bind
+
+
 def check(rc, what):
     if rc != 0:
         raise AgentsAmdError(f"{what} failed: {_ERRORS.get(rc, rc)}")

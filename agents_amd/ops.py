@@ -847,126 +847,19 @@ def dense_loss_head_ok(B, A, mask_src):
 
 
 # ---- policies over many discrete actions (tokens) ---------------------------------------------
-DTYPES = {torch.float32: _lib.AA_DT_F32, torch.bfloat16: _lib.AA_DT_BF16,
-          torch.float16: _lib.AA_DT_F16}
+# Checks, outputs, strides and scratch of these operators are compiled (csrc/token_ops_bind.cpp):
+# in Python they cost several times what the kernels of a small call take.
+_token_ops = None
 
 
-def _one_stride(shape, strides):
-    """Stride of the row index when the axes `shape` fold to one, else None."""
-    stride = rows = None
-    for n, st in zip(reversed(shape), reversed(strides)):
-        if n == 1:
-            continue
-        if stride is None:
-            stride, rows = st, n
-        elif st == stride * rows:
-            rows *= n
-        else:
-            return None
-    return 0 if stride is None else stride
-
-
-def _fold_rows(lead, tensors):
-    """(inner, [(outer stride, inner stride)]) of tensors that share the leading axes `lead`: row r
-    of each starts at (r // inner) * outer + (r % inner) * inner stride (elements).  One stride where
-    every tensor allows it, else the last leading axis keeps one of its own (a [B, T - 1] slice of
-    [B, T] rows); ValueError beyond that."""
-    n = len(lead)
-    if n == 1:
-        return 1, [(0, 0) if t is None else (t.stride(0), 0) for t in tensors]
-    if lead.numel() == 0:
-        return 1, [(0, 0)] * len(tensors)
-    one = [0 if t is None else _one_stride(lead, t.stride()[:n]) for t in tensors]
-    if None not in one:
-        return 1, [(s, 0) for s in one]
-    out = []
-    for t in tensors:
-        s = 0 if t is None else _one_stride(lead[:-1], t.stride()[:n - 1])
-        if s is None:
-            raise ValueError(f"leading axes {tuple(lead)} with strides {t.stride()[:n]} do not fold "
-                             "to two axes; pass a contiguous tensor")
-        out.append((s, 0 if t is None else t.stride(n - 1)))
-    return lead[-1], out
-
-
-def _same_device(t, *others):
-    require_cuda(t, *others)
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"tensors on {t.device} and {o.device}")
-
-
-class _on_device:
-    """Runs a launch on `device`, and on torch's current stream of it, whichever device is current."""
-    __slots__ = ("_ctx",)
-
-    def __init__(self, device):
-        self._ctx = None if device.index == torch.cuda.current_device() else \
-            torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-        return False
-
-
-def _call_scratch(nbytes, device):
-    """Scratch of ONE call from torch's allocator: calls on several streams and captured graphs that
-    replay beside each other never meet in it (a captured call's stays with its graph's pool)."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+def _bind():
+    global _token_ops
+    _token_ops = _lib.load_token_ops()
+    return _token_ops
 
 
 CategoricalLogProb = collections.namedtuple(
     "CategoricalLogProb", ("log_prob", "entropy", "top_ids", "top_log_prob", "stats"))
-
-
-def _expand_mask(mask, logits, what):
-    """`mask` as a view of the logits' shape; its last axis is the actions'."""
-    lead = mask.shape[:-1]
-    if mask.dim() < 1 or mask.dim() > logits.dim() or mask.shape[-1] != logits.shape[-1] or \
-            any(m not in (1, n) for m, n in zip(reversed(lead), reversed(logits.shape[:-1]))):
-        raise ValueError(f"{what}: mask {tuple(mask.shape)} for logits {tuple(logits.shape)}")
-    return mask.expand(logits.shape)
-
-
-def _categorical_desc(logits, actions, mask, temperature, first_action, what):
-    if logits.dim() < 2 or logits.dtype not in DTYPES:
-        raise ValueError(f"{what}: logits must be a float32 / bfloat16 / float16 [.., actions] "
-                         f"tensor, got {logits.dtype} {tuple(logits.shape)}")
-    vocab = logits.shape[-1]
-    if vocab < 1:
-        raise ValueError(f"{what}: no actions")
-    if vocab > 1 and logits.stride(-1) != 1:
-        raise ValueError(f"{what}: the last axis of logits must be contiguous")
-    lead = logits.shape[:-1]
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"{what}: temperature must be positive (1e-30 .. 1e30), got {temperature}")
-    if actions is not None:
-        if actions.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{what}: actions must be int32 or int64, got {actions.dtype}")
-        if actions.shape != lead:
-            raise ValueError(f"{what}: actions {tuple(actions.shape)} for logits "
-                             f"{tuple(logits.shape)}")
-    if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8, torch.int32):
-            raise ValueError(f"{what}: mask must be bool, uint8 or int32, got {mask.dtype}")
-        if mask.shape != logits.shape:
-            mask = _expand_mask(mask, logits, what)
-        if vocab > 1 and mask.stride(-1) != 1:
-            raise ValueError(f"{what}: the last axis of mask must be contiguous")
-    _same_device(logits, actions, mask)
-    inner, ((xo, xi), (ao, ai), (ko, ki)) = _fold_rows(lead, (logits, actions, mask))
-    d = _lib.CategoricalDesc(
-        lead.numel(), inner, vocab, logits.data_ptr(), xo, xi,
-        None if actions is None else actions.data_ptr(), ao, ai, first_action,
-        None if mask is None else mask.data_ptr(), ko, ki, DTYPES[logits.dtype],
-        4 if actions is None else actions.element_size(),
-        1 if mask is None else mask.element_size(), 0, temperature)
-    return d, lead
 
 
 def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k=0, first_action=0):
@@ -980,29 +873,10 @@ def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k
     index past the end gives NaN.  A row whose mask leaves no finite logit: log_prob -inf, entropy 0.
     Returns CategoricalLogProb: log_prob, entropy [..] float32, top_ids [.., k] int64 and
     top_log_prob [.., k] float32 with k = min(top_k, A) (None for top_k=0; equal logits by lower
-    index, -1 / -inf where fewer actions have a probability), and `stats` for the backward call."""
-    what = "categorical_log_prob"
-    d, lead = _categorical_desc(logits, actions, mask, temperature, first_action, what)
-    if not 0 <= top_k <= _lib.AA_CATEGORICAL_MAX_TOP:
-        raise ValueError(f"{what}: top_k must be 0..{_lib.AA_CATEGORICAL_MAX_TOP}, got {top_k}")
-    dev, k = logits.device, min(top_k, logits.shape[-1])
-    log_prob = None if actions is None else torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    stats = torch.empty(lead + (2,), dtype=torch.float32, device=dev)
-    ids = top = None
-    if k > 0:
-        ids = torch.empty(lead + (k,), dtype=torch.int64, device=dev)
-        top = torch.empty(lead + (k,), dtype=torch.float32, device=dev)
-        d.top_ids, d.top_log_prob, d.top_k = ids.data_ptr(), top.data_ptr(), k
-    if d.rows > 0:
-        lib = _lib.load()
-        d.log_prob, d.entropy, d.stats = ptr(log_prob), entropy.data_ptr(), stats.data_ptr()
-        need = lib.aa_categorical_workspace_bytes(ctypes.byref(d))
-        ws = _call_scratch(need, dev)
-        with _on_device(dev):
-            check(lib.aa_categorical_log_prob(ctypes.byref(d), ptr(ws), need, stream_ptr()),
-                  "aa_categorical_log_prob")
-    return CategoricalLogProb(log_prob, entropy, ids, top, stats)
+    index, -1 / -inf where fewer actions have a probability; ids index A, without first_action), and
+    `stats` for the backward call."""
+    return CategoricalLogProb(*(_token_ops or _bind()).categorical_log_prob(
+        logits, actions, mask, temperature, top_k, first_action))
 
 
 def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dentropy=None, mask=None,
@@ -1011,156 +885,38 @@ def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dent
     None); `forward` is what categorical_log_prob returned for the same logits, actions, mask,
     temperature and first_action.  Masked actions and padding rows get 0.  The result has the logits'
     type; `out` may be the logits' own tensor."""
-    what = "categorical_log_prob_backward"
-    d, lead = _categorical_desc(logits, actions, mask, temperature, first_action, what)
-    if dlog_prob is None and dentropy is None:
-        raise ValueError(f"{what}: needs dlog_prob or dentropy")
-    if dlog_prob is not None and actions is None:
-        raise ValueError(f"{what}: dlog_prob needs actions")
-    grads = []
-    for g, name in ((dlog_prob, "dlog_prob"), (dentropy, "dentropy")):
-        if g is not None and (g.dtype != torch.float32 or g.shape != lead):
-            raise ValueError(f"{what}: {name} must be float32 {tuple(lead)}, got {g.dtype} "
-                             f"{tuple(g.shape)}")
-        grads.append(g if g is None or g.is_contiguous() else g.contiguous())
-    entropy, stats = forward.entropy, forward.stats
-    for t, shape, name in ((entropy, lead, "entropy"), (stats, lead + (2,), "stats")):
-        if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError(f"{what}: forward.{name} is not of these logits")
-    if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif out.dtype != logits.dtype or out.shape != logits.shape or \
-            (out.shape[-1] > 1 and out.stride(-1) != 1):
-        raise ValueError(f"{what}: out must be {logits.dtype} {tuple(logits.shape)} with a "
-                         "contiguous last axis")
-    _same_device(logits, grads[0], grads[1], entropy, stats, out)
-    if d.rows == 0:
-        return out
-    d.entropy, d.stats = entropy.data_ptr(), stats.data_ptr()
-    # one fold for all of them
-    d.inner, ((d.x_outer, d.x_inner), (d.a_outer, d.a_inner), (d.k_outer, d.k_inner),
-              (oo, oi)) = _fold_rows(lead, (logits, actions,
-                                            None if mask is None else mask.expand(logits.shape),
-                                            out))
-    with _on_device(logits.device):
-        check(_lib.load().aa_categorical_log_prob_backward(
-            ctypes.byref(d), ptr(grads[0]), ptr(grads[1]), out.data_ptr(), oo, oi, stream_ptr()),
-            "aa_categorical_log_prob_backward")
-    return out
+    return (_token_ops or _bind()).categorical_log_prob_backward(
+        logits, actions, forward.entropy, forward.stats, dlog_prob, dentropy, mask, temperature,
+        first_action, out)
 
 
 # ---- clipping of many gradient tensors ------------------------------------------------------------
-def _clip_tensors(tensors, clip_norm, each, scale, out, what):
-    tensors = list(tensors)
-    n = len(tensors)
-    if n == 0:
-        raise ValueError(f"{what}: no tensors")
-    if scale and not clip_norm > 0:
-        raise ValueError(f"{what}: clip_norm must be positive, got {clip_norm}")
-    t0 = tensors[0]
-    if t0.dtype not in DTYPES:
-        raise ValueError(f"{what}: tensors must be float32 / bfloat16 / float16, got {t0.dtype}")
-    dev, dtype = t0.device, t0.dtype
-    for t in tensors:
-        if t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"{what}: tensors must be contiguous and of one type, got {t.dtype} "
-                             f"{tuple(t.shape)} strides {t.stride()} beside {dtype}")
-        if t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    require_cuda(t0)
-    dst = None
-    if scale:
-        if out is None:
-            out = [torch.empty_like(t) for t in tensors]
-        else:
-            out = list(out)
-            if len(out) != n or any(o.dtype != dtype or o.shape != t.shape or o.device != dev or
-                                    not o.is_contiguous() for o, t in zip(out, tensors)):
-                raise ValueError(f"{what}: out must mirror the tensors")
-        dst = (ctypes.c_void_p * n)(*[o.data_ptr() for o in out])
-    src = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    lib = _lib.load()
-    norm = torch.empty((n,) if each else (), dtype=torch.float32, device=dev)
-    need = lib.aa_clip_tensors_workspace_bytes(sizes, n)
-    ws = _call_scratch(need, dev)
-    with _on_device(dev):
-        check(lib.aa_clip_tensors(src, dst, sizes, n, DTYPES[dtype], float(clip_norm), int(each),
-                                  norm.data_ptr(), ptr(ws), need, stream_ptr()), "aa_clip_tensors")
-    return out, norm
-
-
 def clip_by_global_norm(tensors, clip_norm, out=None):
     """tf.clip_by_global_norm: ([t * clip_norm / max(global norm, clip_norm)], global norm) of a list
-    of contiguous tensors of one type (csrc/grad_clip.hip).  `out`: a list that receives the clipped
-    tensors, `tensors` itself for clipping in place.  The norm is a float32 scalar on the device; one
-    that is not finite makes every clipped value NaN."""
-    return _clip_tensors(tensors, clip_norm, False, True, out, "clip_by_global_norm")
+    of contiguous float32 / bfloat16 / float16 tensors of one type (csrc/grad_clip.hip).  `out`: a
+    list that receives the clipped tensors, `tensors` itself for clipping in place.  The norm is a
+    float32 scalar on the device; one that is not finite makes every clipped value NaN."""
+    return (_token_ops or _bind()).clip(tensors, clip_norm, False, True, out, "clip_by_global_norm")
 
 
 def clip_by_norms(tensors, clip_norm, out=None):
     """tf.clip_by_norm of every tensor by itself: ([t * clip_norm / max(norm of t, clip_norm)],
     norms [n] float32)."""
-    return _clip_tensors(tensors, clip_norm, True, True, out, "clip_by_norms")
+    return (_token_ops or _bind()).clip(tensors, clip_norm, True, True, out, "clip_by_norms")
 
 
 def global_norm(tensors):
     """tf.linalg.global_norm of a list of tensors: float32 scalar on the device."""
-    return _clip_tensors(tensors, 1.0, False, False, None, "global_norm")[1]
+    return (_token_ops or _bind()).clip(tensors, 0.0, False, False, None, "global_norm")[1]
 
 
 # ---- layer normalisation ----------------------------------------------------------------------------
-def _norm_rows(t, name, shape, dtype, what):
-    if t.dtype != dtype or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
-        raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)} with a contiguous last "
-                         f"axis, got {t.dtype} {tuple(t.shape)} strides {t.stride()}")
-
-
-def _norm_weight(w, name, width, what):
-    if w is not None and (w.dtype != torch.float32 or w.shape != (width,) or
-                          not w.is_contiguous()):
-        raise ValueError(f"{what}: {name} must be contiguous float32 [{width}], got {w.dtype} "
-                         f"{tuple(w.shape)}")
-
-
-def _norm_check(x, gamma, what):
-    if x.dim() < 2 or x.dtype not in DTYPES or x.shape[-1] < 1:
-        raise ValueError(f"{what}: x must be a float32 / bfloat16 / float16 [.., n] tensor, got "
-                         f"{x.dtype} {tuple(x.shape)}")
-    _norm_rows(x, "x", x.shape, x.dtype, what)
-    _norm_weight(gamma, "gamma", x.shape[-1], what)
-
-
 def layer_norm_forward(x, gamma, beta, epsilon=1e-3, out=None, stats=None):
     """keras LayerNormalization over the last axis: (x - mean) / sqrt(var + epsilon) * gamma + beta
     (csrc/layer_norm.hip).  x [.., n] float32 / bfloat16 / float16; gamma, beta float32 [n] or None.
     Returns (y, stats): y in x's type, stats [.., 2] float32 (mean, 1 / sqrt(var + epsilon)) for the
     backward call.  `out` may be x."""
-    what = "layer_norm_forward"
-    _norm_check(x, gamma, what)
-    _norm_weight(beta, "beta", x.shape[-1], what)
-    if not epsilon >= 0:
-        raise ValueError(f"{what}: epsilon must not be negative, got {epsilon}")
-    lead = x.shape[:-1]
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _norm_rows(out, "out", x.shape, x.dtype, what)
-    if stats is None:
-        stats = torch.empty(lead + (2,), dtype=torch.float32, device=x.device)
-    elif stats.shape != lead + (2,) or stats.dtype != torch.float32 or not stats.is_contiguous():
-        raise ValueError(f"{what}: stats must be contiguous float32 {tuple(lead) + (2,)}")
-    _same_device(x, gamma, beta, out, stats)
-    rows = lead.numel()
-    if rows > 0:
-        inner, ((xo, xi), (yo, yi)) = _fold_rows(lead, (x, out))
-        d = _lib.LayerNormDesc(rows, inner, x.shape[-1], x.data_ptr(), xo, xi, None, 0, 0,
-                               out.data_ptr(), yo, yi, None, 0, 0, ptr(gamma), ptr(beta),
-                               stats.data_ptr(), None, None, epsilon, DTYPES[x.dtype])
-        with _on_device(x.device):
-            check(_lib.load().aa_layer_norm_forward(ctypes.byref(d), stream_ptr()),
-                  "aa_layer_norm_forward")
-    return out, stats
+    return (_token_ops or _bind()).layer_norm_forward(x, gamma, beta, epsilon, out, stats)
 
 
 def layer_norm_backward(dy, x, gamma, stats, dx=None, dgamma=None, dbeta=None, mask_act=None,
@@ -1169,46 +925,8 @@ def layer_norm_backward(dy, x, gamma, stats, dx=None, dgamma=None, dbeta=None, m
     (overwritten; given buffers are filled).  `mask_act`: dx is multiplied by that activation's
     derivative, x being its output (as dense_dx's).  param_grads=False / input_grad=False leave out
     the weights' / the input's gradient (None in the result).  `dx` may be x or dy."""
-    what = "layer_norm_backward"
-    _norm_check(x, gamma, what)
-    lead, width = x.shape[:-1], x.shape[-1]
-    _norm_rows(dy, "dy", x.shape, x.dtype, what)
-    if stats.shape != lead + (2,) or stats.dtype != torch.float32 or not stats.is_contiguous():
-        raise ValueError(f"{what}: stats must be contiguous float32 {tuple(lead) + (2,)}")
-    if not (param_grads or input_grad):
-        raise ValueError(f"{what}: nothing to compute")
-    dev = x.device
-    if not input_grad:
-        dx = None
-    elif dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    else:
-        _norm_rows(dx, "dx", x.shape, x.dtype, what)
-    if param_grads:
-        dgamma = torch.empty(width, dtype=torch.float32, device=dev) if dgamma is None else dgamma
-        dbeta = torch.empty(width, dtype=torch.float32, device=dev) if dbeta is None else dbeta
-        _norm_weight(dgamma, "dgamma", width, what)
-        _norm_weight(dbeta, "dbeta", width, what)
-    else:
-        dgamma = dbeta = None
-    _same_device(x, dy, gamma, stats, dx, dgamma, dbeta)
-    rows = lead.numel()
-    if rows == 0:
-        if param_grads:
-            dgamma.zero_()
-            dbeta.zero_()
-        return dx, dgamma, dbeta
-    lib = _lib.load()
-    inner, ((xo, xi), (go, gi), (do, di)) = _fold_rows(lead, (x, dy, dx))
-    d = _lib.LayerNormDesc(rows, inner, width, x.data_ptr(), xo, xi, dy.data_ptr(), go, gi, None,
-                           0, 0, ptr(dx), do, di, ptr(gamma), None, stats.data_ptr(), ptr(dgamma),
-                           ptr(dbeta), 0.0, DTYPES[x.dtype], ACT[mask_act])
-    need = lib.aa_layer_norm_backward_workspace_bytes(ctypes.byref(d))
-    ws = _call_scratch(need, dev)
-    with _on_device(dev):
-        check(lib.aa_layer_norm_backward(ctypes.byref(d), ptr(ws), need, stream_ptr()),
-              "aa_layer_norm_backward")
-    return dx, dgamma, dbeta
+    return (_token_ops or _bind()).layer_norm_backward(
+        dy, x, gamma, stats, dx, dgamma, dbeta, ACT[mask_act], bool(param_grads), bool(input_grad))
 
 
 __all__ = [n for n in dir() if not n.startswith("_")]

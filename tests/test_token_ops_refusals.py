@@ -7,6 +7,9 @@ import torch
 from agents_amd import _lib, ops
 
 
+pytestmark = pytest.mark.usefixtures("lib")
+
+
 def bad(fn, *a, **kw):
     with pytest.raises((ValueError, _lib.AgentsAmdError)):
         fn(*a, **kw)
