@@ -16,6 +16,7 @@
 #include "common.h"
 #include "agents_amd.h"
 #include "vec_types.h"
+#include "wave_ops.h"
 
 #define CAT_MARGIN 4.f             // powers of two a value may exceed its lane's reference by
 #define CAT_LOWEST (-3.402823466e+38f)
@@ -43,7 +44,7 @@ struct CatArgs {
   float* top_log_prob;
   int splits;                      // parts of a row
   float* part;                     // [rows][splits][4]
-  u64* part_keys;                  // [rows][splits][top_k]
+  u64* part_keys;                  // [rows][top_k][splits]
 };
 
 struct CatSum {
@@ -73,12 +74,12 @@ __device__ static inline CatSum cat_join(CatSum a, CatSum b, float c2) {
   return a;
 }
 
-__device__ static inline CatSum cat_shfl_xor(CatSum a, int m) {
-  CatSum o;
-  o.r = __shfl_xor(a.r, m, 64);
-  o.s = __shfl_xor(a.s, m, 64);
-  o.t = __shfl_xor(a.t, m, 64);
-  return o;
+// the triples of a wave's lanes, in every lane
+__device__ static inline CatSum cat_wave_join(CatSum a, float c2) {
+  a = cat_move(a, wv_max(a.r), c2);
+  a.s = wv_sum(a.s);
+  a.t = wv_sum(a.t);
+  return a;
 }
 
 // ---- alternatives: keys that order as (value, then lower index) ---------------------------------
@@ -93,28 +94,10 @@ __device__ static inline float cat_key_value(u64 k) {
 }
 __device__ static inline int cat_key_index(u64 k) { return (int)~(unsigned)k; }
 
-__device__ static inline u64 cat_sort_desc(u64 v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const u64 o = __shfl_xor(v, j, 64);
-      const bool larger = ((lane & j) == 0) == ((lane & k) == 0);
-      v = (larger == (v > o)) ? v : o;
-    }
-  return v;
-}
-
-// the 64 best of two descending lists
-__device__ static inline u64 cat_merge_desc(u64 a, u64 b, int lane) {
-  const u64 r = __shfl(b, 63 - lane, 64);
-  u64 v = a > r ? a : r;
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) {
-    const u64 o = __shfl_xor(v, j, 64);
-    v = (((lane & j) == 0) == (v > o)) ? v : o;
-  }
-  return v;
+__device__ static inline u64 cat_lane(u64 v, int from) {       // `from` is wave-uniform
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)v, from);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(v >> 32), from);
+  return ((u64)hi << 32) | lo;
 }
 
 struct CatTop {
@@ -132,8 +115,8 @@ __device__ static inline void cat_wave_fence() {
 }
 
 __device__ static inline void cat_top_merge(CatTop& t, u64 cand, int lane, int k) {
-  t.list = cat_merge_desc(t.list, cat_sort_desc(cand, lane), lane);
-  const u64 kth = __shfl(t.list, k - 1, 64);
+  t.list = wv_merge_desc(t.list, wv_sort_desc(cand, lane, true), lane);
+  const u64 kth = cat_lane(t.list, k - 1);
   if (kth > t.bar) t.bar = kth;
 }
 
@@ -229,10 +212,62 @@ __device__ static inline void cat_pad_row(const CatArgs& a, int64_t row, int lan
   }
 }
 
+// U chunks of a lane, TEAM apart, and their masks: all loads in flight together
+template <typename T, int MB, int U>
+struct CatTile {
+  static constexpr int C = T::C;
+  static constexpr int W = MB == 0 ? 1 : MB * C / 4;       // mask words of a chunk
+  uint4 q[U];
+  unsigned m[U][W];
+};
+
+template <typename T, int MB, int U>
+__device__ static inline void cat_load(const typename T::elem* x, const uint8_t* mk, int k, int team,
+                                       int k1, int skew, int vocab, CatTile<T, MB, U>& t) {
+  constexpr int C = T::C;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int ku = k + u * team, e0 = ku * C - skew;
+    t.q[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (ku < k1 && e0 >= 0 && e0 + C <= vocab) {
+      t.q[u] = vt_load16(x + e0);
+      if (MB != 0) __builtin_memcpy(t.m[u], mk + (int64_t)MB * e0, MB * C);
+    }
+  }
+}
+
+// chunk u as fp32, -inf where it is masked or not there
+template <typename T, int MB, int U>
+__device__ static inline void cat_values(const typename T::elem* x, const uint8_t* mk, int ku, int k1,
+                                         int skew, int vocab, const CatTile<T, MB, U>& t, int u,
+                                         float (&v)[T::C]) {
+  constexpr int C = T::C;
+  const int e0 = ku * C - skew;
+  if (ku < k1 && e0 >= 0 && e0 + C <= vocab) {
+    T::widen(t.q[u], v);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if (MB == 1 && ((t.m[u][j / 4] >> (8 * (j % 4))) & 0xffu) == 0u) v[j] = -INFINITY;
+      if (MB == 4 && t.m[u][j] == 0u) v[j] = -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int e = e0 + j;
+      v[j] = -INFINITY;
+      if (ku < k1 && e >= 0 && e < vocab) {
+        v[j] = T::one(x[e]);
+        if (MB == 1 && mk[e] == 0) v[j] = -INFINITY;
+        if (MB == 4 && reinterpret_cast<const int32_t*>(mk)[e] == 0) v[j] = -INFINITY;
+      }
+    }
+  }
+}
+
 // TEAM = 64: a wave per row, four rows per workgroup.  TEAM = 256: a workgroup per part of a row.
 template <typename T, int MB, int TEAM, bool TOP>
 __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
-  constexpr int C = T::C;
+  constexpr int C = T::C, U = MB == 4 ? 2 : 4;
   __shared__ float red[3][4];
   __shared__ u64 keys[TOP ? 4 : 1][TOP ? 128 : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -242,10 +277,6 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   const int part = TEAM == 64 ? 0 : (int)(item - row * a.splits);
   if (row >= a.rows) return;       // (the whole workgroup, or a wave that meets no barrier)
   const int64_t action = cat_action(a, row);
-  if (action < 0) {
-    if (a.splits == 1) cat_pad_row(a, row, me);
-    return;                                     // the whole team returns; the joining launch writes
-  }
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
                               vt_row(row, a.inner, a.x_outer, a.x_inner);
   const uint8_t* mk = MB == 0 ? nullptr : reinterpret_cast<const uint8_t*>(a.mask) +
@@ -256,81 +287,61 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   const int each = TEAM == 64 ? chunks : (chunks + a.splits - 1) / a.splits;
   const int k0 = part * each;
   const int k1 = k0 + each < chunks ? k0 + each : chunks;
+  const int first = k0 + (TEAM == 64 ? 0 : wave * 64);
+  CatTile<T, MB, U> next;
+  cat_load<T, MB, U>(x, mk, first + lane, TEAM, k1, skew, a.vocab, next);
+  if (action < 0) {
+    if (a.splits == 1) cat_pad_row(a, row, me);
+    return;                        // the whole team returns; the joining launch writes
+  }
   const float c2 = a.inv_t * CAT_LOG2E;
   const float margin = CAT_MARGIN / c2;
   CatSum u = {CAT_LOWEST, 0.f, 0.f};
   CatTop top = {0ull, CAT_EMPTY_KEY, 0, TOP ? keys[wave] : nullptr};
-  for (int kb = k0 + (TEAM == 64 ? 0 : wave * 64); kb < k1; kb += TEAM) {   // (wave-uniform)
-    const int k = kb + lane;
-    const int e0 = k * C - skew;
-    float v[C];
-    if (k < k1 && e0 >= 0 && e0 + C <= a.vocab) {
-      T::widen(vt_load16(x + e0), v);
-      if (MB == 1) {
-        u64 m;
-        if (C == 8) {
-          __builtin_memcpy(&m, mk + e0, 8);
-        } else {
-          unsigned m4;
-          __builtin_memcpy(&m4, mk + e0, 4);
-          m = m4;
-        }
+  for (int kb = first; kb < k1; kb += TEAM * U) {          // (wave-uniform)
+    const CatTile<T, MB, U> tile = next;
+    if (kb + TEAM * U < k1)
+      cat_load<T, MB, U>(x, mk, kb + TEAM * U + lane, TEAM, k1, skew, a.vocab, next);
+    float v[U][C], high[U];
+    float highest = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (((m >> (8 * j)) & 0xffull) == 0ull) v[j] = -INFINITY;
-      }
-      if (MB == 4) {
+    for (int i = 0; i < U; ++i) {
+      cat_values<T, MB, U>(x, mk, kb + i * TEAM + lane, k1, skew, a.vocab, tile, i, v[i]);
+      high[i] = v[i][0];
 #pragma unroll
-        for (int j = 0; j < C; j += 4) {
-          const uint4 m = vt_load16(mk + 4 * (int64_t)(e0 + j));
-          if (m.x == 0u) v[j] = -INFINITY;
-          if (m.y == 0u) v[j + 1] = -INFINITY;
-          if (m.z == 0u) v[j + 2] = -INFINITY;
-          if (m.w == 0u) v[j + 3] = -INFINITY;
-        }
-      }
-    } else {
+      for (int j = 1; j < C; ++j) high[i] = fmaxf(high[i], v[i][j]);
+      highest = fmaxf(highest, high[i]);
+    }
+    if (highest > u.r + margin) u = cat_move(u, highest, c2);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        const int e = e0 + j;
-        v[j] = -INFINITY;
-        if (k < k1 && e >= 0 && e < a.vocab) {
-          v[j] = T::one(x[e]);
-          if (MB == 1 && mk[e] == 0) v[j] = -INFINITY;
-          if (MB == 4 && reinterpret_cast<const int32_t*>(mk)[e] == 0) v[j] = -INFINITY;
-        }
+        const float d = v[i][j] - u.r;
+        const float e = cat_exp2(d * c2);
+        u.s += e;
+        u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
       }
-    }
-    float high = v[0];
-#pragma unroll
-    for (int j = 1; j < C; ++j) high = fmaxf(high, v[j]);
-    if (high > u.r + margin) u = cat_move(u, high, c2);
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const float d = v[j] - u.r;
-      const float e = cat_exp2(d * c2);
-      u.s += e;
-      u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
-    }
     if (TOP) {
-      if (kb == k0 + (TEAM == 64 ? 0 : wave * 64)) {
-        // first round: k lanes have a chunk maximum at or above the k-th of the maxima, so the row's
-        // k best are too
-        const u64 kth = __shfl(cat_sort_desc(cat_key(high, 0), lane), a.top_k - 1, 64);
-        const u64 bar = kth & 0xffffffff00000000ull;
+      if (kb == first) {
+        // k lanes hold a value at or above the k-th of the lanes' maxima, so the row's k best are too
+        const unsigned sorted = wv_sort_desc((unsigned)(cat_key(highest, 0) >> 32), lane);
+        const u64 bar = (u64)(unsigned)__builtin_amdgcn_readlane((int)sorted, a.top_k - 1) << 32;
         if (bar > top.bar) top.bar = bar;
       }
-      if (__any(cat_key(high, 0) > top.bar)) {
 #pragma unroll
-        for (int j = 0; j < C; ++j)
-          cat_top_offer(top, v[j], e0 + j, k < k1 && v[j] > -INFINITY, lane, a.top_k);
-      }
+      for (int i = 0; i < U; ++i)
+        if (__any(cat_key(high[i], 0) > top.bar)) {
+          const int ku = kb + i * TEAM + lane;
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+            cat_top_offer(top, v[i][j], ku * C - skew + j, v[i][j] > -INFINITY, lane, a.top_k);
+        }
     }
   }
   if (TOP)
     while (top.held > 0) cat_top_flush(top, lane, a.top_k);
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) u = cat_join(u, cat_shfl_xor(u, m), c2);
+  u = cat_wave_join(u, c2);
   if constexpr (TEAM == 64) {
     float ls = 0.f;
     if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
@@ -344,7 +355,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
     for (int w = 1; w < 4; ++w) {
       CatSum o = {red[0][w], red[1][w], red[2][w]};
       u = cat_join(u, o, c2);
-      if (TOP) top.list = cat_merge_desc(top.list, keys[w][lane], lane);
+      if (TOP) top.list = wv_merge_desc(top.list, keys[w][63 - lane], lane);
     }
     if (a.splits == 1) {
       float ls = 0.f;
@@ -355,7 +366,9 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
         float* p = a.part + item * 4;
         p[0] = u.r; p[1] = u.s; p[2] = u.t; p[3] = 0.f;
       }
-      if (TOP && lane < a.top_k) a.part_keys[item * a.top_k + lane] = top.list;
+      // the parts' lists interleaved by rank: the first keys that the join reads are the best ones
+      if (TOP && lane < a.top_k)
+        a.part_keys[(row * a.top_k + lane) * a.splits + part] = top.list;
     }
   }
 }
@@ -378,8 +391,7 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
     CatSum o = {q[0], q[1], q[2]};
     u = cat_join(u, o, c2);
   }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) u = cat_join(u, cat_shfl_xor(u, m), c2);
+  u = cat_wave_join(u, c2);
   float ls = 0.f;
   if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
   if (TOP) {

@@ -19,17 +19,21 @@
 #define CLIP_MIN_PIECE 8192        // elements
 #define CLIP_PIECES 2048           // workgroups a large list is cut into: 8 per CU
 #define CLIP_JOIN 4096
+#define CLIP_UNROLL 4
+#define CLIP_FEW 16
 
+template <int N>
 struct ClipList {
-  const void* src[AA_CLIP_TENSORS];
-  void* dst[AA_CLIP_TENSORS];
-  int64_t n[AA_CLIP_TENSORS];
-  uint32_t first[AA_CLIP_TENSORS + 1];   // first workgroup of every tensor
-  int32_t count;
+  const void* src[N];
+  void* dst[N];
+  int64_t n[N];
   int64_t piece;                         // elements per workgroup
+  uint32_t first[N + 1];                 // first workgroup of every tensor
+  int32_t count;
 };
 
-__device__ static inline int clip_find(const ClipList& L, unsigned b) {
+template <int N>
+__device__ static inline int clip_find(const ClipList<N>& L, unsigned b) {
   int lo = 0, hi = L.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -50,26 +54,40 @@ __device__ static inline double clip_block_sum(double v, double* red) {
   return s;
 }
 
-template <typename T>
+// U loads of a lane are in flight at once
+template <typename T, int U>
+__device__ static inline void clip_load(const typename T::elem* g, int64_t c, uint4 (&q)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) q[u] = vt_load16(g + c + (int64_t)u * CLIP_THREADS * T::C);
+}
+
+template <typename T, int N>
 __global__ void __launch_bounds__(CLIP_THREADS)
-aa_clip_sumsq_kernel(ClipList L, double* __restrict__ partial) {
-  constexpr int C = T::C;
+aa_clip_sumsq_kernel(ClipList<N> L, double* __restrict__ partial) {
+  constexpr int C = T::C, U = CLIP_UNROLL, ROUND = CLIP_THREADS * C;
   __shared__ double red[16];
   const int t = clip_find(L, blockIdx.x);
   const int64_t lo = (int64_t)(blockIdx.x - L.first[t]) * L.piece;
   const int64_t n = L.n[t] - lo < L.piece ? L.n[t] - lo : L.piece;
   const typename T::elem* g = reinterpret_cast<const typename T::elem*>(L.src[t]) + lo;
   double s0 = 0.0, s1 = 0.0;
-  int64_t c = (int64_t)threadIdx.x * C;
-  for (; c + C <= n; c += CLIP_THREADS * C) {
+  auto add = [&](const uint4& q) {
     float v[C];
-    T::widen(vt_load16(g + c), v);
+    T::widen(q, v);
 #pragma unroll
     for (int j = 0; j < C; j += 2) {
       s0 = fma((double)v[j], (double)v[j], s0);
       s1 = fma((double)v[j + 1], (double)v[j + 1], s1);
     }
+  };
+  int64_t c = (int64_t)threadIdx.x * C;
+  for (; c + (U - 1) * ROUND + C <= n; c += U * ROUND) {
+    uint4 q[U];
+    clip_load<T, U>(g, c, q);
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(q[u]);
   }
+  for (; c + C <= n; c += ROUND) add(vt_load16(g + c));
   for (int64_t k = c; k < n && k < c + C; ++k) s0 += (double)T::one(g[k]) * (double)T::one(g[k]);
   const double s = clip_block_sum(s0 + s1, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -88,13 +106,23 @@ aa_clip_join_kernel(const double* __restrict__ partial, int64_t count, double* _
   }
 }
 
-template <typename T>
+template <typename T, int N>
 __global__ void __launch_bounds__(CLIP_THREADS)
-aa_clip_scale_kernel(ClipList L, const double* __restrict__ partial, int64_t count, double clip,
+aa_clip_scale_kernel(ClipList<N> L, const double* __restrict__ partial, int64_t count, double clip,
                      int each, float* __restrict__ norm) {
-  constexpr int C = T::C;
+  constexpr int C = T::C, U = CLIP_UNROLL, ROUND = CLIP_THREADS * C;
   __shared__ double red[16];
-  const int t = clip_find(L, blockIdx.x);
+  // the pieces in the opposite order of the first pass: what it read last is still cached
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int t = clip_find(L, block);
+  const int64_t lo = (int64_t)(block - L.first[t]) * L.piece;
+  const int64_t n = L.n[t] - lo < L.piece ? L.n[t] - lo : L.piece;
+  const typename T::elem* g = reinterpret_cast<const typename T::elem*>(L.src[t]) + lo;
+  typename T::elem* o = reinterpret_cast<typename T::elem*>(L.dst[t]) + lo;
+  int64_t c = (int64_t)threadIdx.x * C;
+  bool full = c + (U - 1) * ROUND + C <= n;
+  uint4 q[U];
+  if (full) clip_load<T, U>(g, c, q);          // in flight while the pieces' sums are added
   // `partial` is the list's own in `each` mode, the whole call's otherwise
   const int64_t p0 = each ? L.first[t] : 0, p1 = each ? L.first[t + 1] : count;
   double s = 0.0;
@@ -102,25 +130,28 @@ aa_clip_scale_kernel(ClipList L, const double* __restrict__ partial, int64_t cou
   const double nrm = sqrt(clip_block_sum(s, red));
   if (threadIdx.x == 0 && norm != nullptr) {
     if (each) {
-      if (blockIdx.x == L.first[t]) norm[t] = (float)nrm;
-    } else if (blockIdx.x == 0) {
+      if (block == L.first[t]) norm[t] = (float)nrm;
+    } else if (block == 0) {
       norm[0] = (float)nrm;
     }
   }
   // the factor is rounded to fp32 once; no clipping gives exactly 1
   const float f = nrm <= clip ? 1.f : isfinite(nrm) ? (float)(clip / nrm) : NAN;
-  const int64_t lo = (int64_t)(blockIdx.x - L.first[t]) * L.piece;
-  const int64_t n = L.n[t] - lo < L.piece ? L.n[t] - lo : L.piece;
-  const typename T::elem* g = reinterpret_cast<const typename T::elem*>(L.src[t]) + lo;
-  typename T::elem* o = reinterpret_cast<typename T::elem*>(L.dst[t]) + lo;
-  int64_t c = (int64_t)threadIdx.x * C;
-  for (; c + C <= n; c += CLIP_THREADS * C) {
+  auto put = [&](const uint4& q, int64_t at) {
     float v[C];
-    T::widen(vt_load16(g + c), v);
+    T::widen(q, v);
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] *= f;
-    vt_store16(o + c, T::pack(v));
+    vt_store16(o + at, T::pack(v));
+  };
+  while (full) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) put(q[u], c + u * ROUND);
+    c += U * ROUND;
+    full = c + (U - 1) * ROUND + C <= n;
+    if (full) clip_load<T, U>(g, c, q);
   }
+  for (; c + C <= n; c += ROUND) put(vt_load16(g + c), c);
   for (int64_t k = c; k < n && k < c + C; ++k) o[k] = T::put(T::one(g[k]) * f);
 }
 
@@ -146,15 +177,64 @@ static int clip_check(const int64_t* n_h, int32_t n_tensors, int32_t dtype) {
   return AA_OK;
 }
 
-template <typename T>
-static void clip_launch(const ClipList& L, unsigned blocks, bool scale, const double* partial,
+template <typename T, int N>
+static void clip_launch(const ClipList<N>& L, unsigned blocks, bool scale, const double* partial,
                         int64_t count, double clip, int each, float* norm, hipStream_t st) {
   if (scale)
-    aa_clip_scale_kernel<T><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(L, partial, count, clip,
-                                                                         each, norm);
+    aa_clip_scale_kernel<T, N><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(L, partial, count, clip,
+                                                                            each, norm);
   else
-    aa_clip_sumsq_kernel<T><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(
+    aa_clip_sumsq_kernel<T, N><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(
         L, const_cast<double*>(partial));
+}
+
+struct ClipCall {
+  const void* const* src;
+  void* const* dst;                // null: the global norm only
+  const int64_t* n;
+  int32_t n_tensors, dtype, each;
+  int64_t piece, total;            // elements of a piece, pieces of the call
+  double clip;
+  float* norm;
+  double* joined;
+  double* partial;
+};
+
+template <int N>
+static void clip_run(const ClipCall& c, hipStream_t st) {
+  for (int pass = 0; pass < (c.dst != nullptr ? 2 : 1); ++pass) {
+    int64_t done = 0;
+    for (int32_t base = 0; base < c.n_tensors; base += N) {
+      ClipList<N> L;
+      L.count = c.n_tensors - base < N ? c.n_tensors - base : N;
+      L.piece = c.piece;
+      uint32_t blocks = 0;
+      for (int i = 0; i < N; ++i) {
+        const bool in = i < L.count;
+        L.src[i] = in ? c.src[base + i] : nullptr;
+        L.dst[i] = in && c.dst != nullptr ? c.dst[base + i] : nullptr;
+        L.n[i] = in ? c.n[base + i] : 0;
+        L.first[i] = blocks;
+        if (in) blocks += (uint32_t)clip_pieces_of(L.n[i], c.piece);
+      }
+      L.first[N] = blocks;
+      const double* sums = c.partial;
+      int64_t count = c.total;
+      if (pass == 0 || c.each) sums = c.partial + done;
+      else if (c.total > CLIP_JOIN) { sums = c.joined; count = 1; }
+      float* nrm = c.each ? c.norm + base : (base == 0 ? c.norm : nullptr);
+      if (c.dtype == AA_DT_F32)
+        clip_launch<VtF32, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+      else if (c.dtype == AA_DT_BF16)
+        clip_launch<VtBf16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+      else
+        clip_launch<VtF16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+      done += blocks;
+    }
+    if (pass == 0 && !c.each && (c.dst == nullptr || c.total > CLIP_JOIN))
+      aa_clip_join_kernel<<<dim3(1), dim3(1024), 0, st>>>(c.partial, c.total, c.joined,
+                                                          c.dst == nullptr ? c.norm : nullptr);
+  }
 }
 
 extern "C" {
@@ -180,46 +260,13 @@ int aa_clip_tensors(const void* const* src_h, void* const* dst_h, const int64_t*
       return AA_ERR_INVALID;
   if (workspace == nullptr || workspace_bytes < aa_clip_tensors_workspace_bytes(n_h, n_tensors))
     return AA_ERR_RANGE;
-  const int64_t piece = clip_piece(n_h, n_tensors);
-  double* joined = (double*)workspace;
-  double* partial = joined + 1;
-  hipStream_t st = (hipStream_t)stream;
-  int64_t total = 0;
-  for (int32_t i = 0; i < n_tensors; ++i) total += clip_pieces_of(n_h[i], piece);
-  if (total > 0x7fffffff) return AA_ERR_RANGE;
-  for (int pass = 0; pass < (scale ? 2 : 1); ++pass) {
-    int64_t done = 0;
-    for (int32_t base = 0; base < n_tensors; base += AA_CLIP_TENSORS) {
-      ClipList L;
-      L.count = n_tensors - base < AA_CLIP_TENSORS ? n_tensors - base : AA_CLIP_TENSORS;
-      L.piece = piece;
-      uint32_t blocks = 0;
-      for (int i = 0; i < AA_CLIP_TENSORS; ++i) {
-        const bool in = i < L.count;
-        L.src[i] = in ? src_h[base + i] : nullptr;
-        L.dst[i] = in && scale ? dst_h[base + i] : nullptr;
-        L.n[i] = in ? n_h[base + i] : 0;
-        L.first[i] = blocks;
-        if (in) blocks += (uint32_t)clip_pieces_of(L.n[i], piece);
-      }
-      L.first[AA_CLIP_TENSORS] = blocks;
-      const double* sums = partial;
-      int64_t count = total;
-      if (pass == 0 || each) sums = partial + done;
-      else if (total > CLIP_JOIN) { sums = joined; count = 1; }
-      float* nrm = each ? norm + base : (base == 0 ? norm : nullptr);
-      if (dtype == AA_DT_F32)
-        clip_launch<VtF32>(L, blocks, pass == 1, sums, count, clip, each, nrm, st);
-      else if (dtype == AA_DT_BF16)
-        clip_launch<VtBf16>(L, blocks, pass == 1, sums, count, clip, each, nrm, st);
-      else
-        clip_launch<VtF16>(L, blocks, pass == 1, sums, count, clip, each, nrm, st);
-      done += blocks;
-    }
-    if (pass == 0 && !each && (!scale || total > CLIP_JOIN))
-      aa_clip_join_kernel<<<dim3(1), dim3(1024), 0, st>>>(partial, total, joined,
-                                                          scale ? nullptr : norm);
-  }
+  ClipCall c = {src_h, dst_h, n_h, n_tensors, dtype, each != 0, clip_piece(n_h, n_tensors), 0, clip,
+                norm, (double*)workspace, (double*)workspace + 1};
+  for (int32_t i = 0; i < n_tensors; ++i) c.total += clip_pieces_of(n_h[i], c.piece);
+  if (c.total > 0x7fffff) return AA_ERR_RANGE;
+  // the arguments of a launch are written by the host for every call: a short list for few tensors
+  if (n_tensors <= CLIP_FEW) clip_run<CLIP_FEW>(c, (hipStream_t)stream);
+  else clip_run<AA_CLIP_TENSORS>(c, (hipStream_t)stream);
   return aa_launch_status();
 }
 

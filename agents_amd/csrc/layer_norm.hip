@@ -14,6 +14,7 @@
 #include "common.h"
 #include "agents_amd.h"
 #include "vec_types.h"
+#include "wave_ops.h"
 
 #define LN_MAX_WIDTH_REG 16384
 #define LN_PER_LANE 16
@@ -34,7 +35,7 @@ struct LnArgs {
 
 template <int TEAM>
 __device__ static inline float ln_team_sum(float v, float* red) {
-  v = vt_wave_sum_all(v);
+  v = wv_sum(v);
   if constexpr (TEAM == 64) return v;
   constexpr int NW = TEAM / 64;
   __syncthreads();
@@ -49,8 +50,8 @@ __device__ static inline float ln_team_sum(float v, float* red) {
 // two sums behind one pair of barriers
 template <int TEAM>
 __device__ static inline void ln_team_sum2(float& a, float& b, float* red) {
-  a = vt_wave_sum_all(a);
-  b = vt_wave_sum_all(b);
+  a = wv_sum(a);
+  b = wv_sum(b);
   if constexpr (TEAM == 64) return;
   constexpr int NW = TEAM / 64;
   __syncthreads();
@@ -103,57 +104,65 @@ __device__ static inline void ln_load_weight(const float* w, int lane, int team,
   }
 }
 
+// A team walks rows `stride` apart: the weights are read once, the next row's loads are in flight while
+// this one is worked on.
 template <typename T, int TEAM, int NCH>
 __global__ void __launch_bounds__(TEAM == 64 ? 256 : TEAM)
 aa_layer_norm_fwd_kernel(LnArgs a) {
   constexpr int C = T::C;
+  constexpr int PER = TEAM == 64 ? 4 : 1;        // teams of a workgroup
   __shared__ float red[32];
-  const int64_t row = TEAM == 64 ? vt_block() * 4 + (threadIdx.x >> 6) : vt_block();
+  const int64_t row0 = (int64_t)blockIdx.x * PER + (TEAM == 64 ? threadIdx.x >> 6 : 0);
+  const int64_t stride = (int64_t)gridDim.x * PER;
   const int lane = TEAM == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  if (row >= a.rows) return;       // (the whole workgroup, or a wave that meets no barrier)
-  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x) +
-                              vt_row(row, a.inner, a.x_outer, a.x_inner);
-  uint4 q[NCH];
-  ln_load<T, NCH>(x, lane, TEAM, a.width, q);
-  float v[NCH][C];
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    T::widen(q[i], v[i]);
-#pragma unroll
-    for (int j = 0; j < C; ++j) s += v[i][j];
-  }
-  // (a quotient, not a product with 1 / D: a constant row's mean is its value, its y is beta)
-  const float width = (float)a.width;
-  const float mean = ln_team_sum<TEAM>(s, red) / width;
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int n = a.width - (lane + i * TEAM) * C;
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      v[i][j] -= mean;
-      ss += j < n ? v[i][j] * v[i][j] : 0.f;
-    }
-  }
-  const float var = ln_team_sum<TEAM>(ss, red) / width;
-  const float rstd = 1.f / sqrtf(var + a.epsilon);
-  if (lane == 0 && a.stats != nullptr) {
-    a.stats[2 * row] = mean;
-    a.stats[2 * row + 1] = rstd;
-  }
+  if (row0 >= a.rows) return;      // (the whole workgroup, or a wave that meets no barrier)
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x);
+  typename T::elem* out = reinterpret_cast<typename T::elem*>(a.out);
+  uint4 next[NCH];
+  ln_load<T, NCH>(x + vt_row(row0, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, next);
   float gm[NCH][C], bt[NCH][C];
   ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
   ln_load_weight<C, NCH>(a.beta, lane, TEAM, a.width, 0.f, bt);
-  typename T::elem* y = reinterpret_cast<typename T::elem*>(a.out) +
-                        vt_row(row, a.inner, a.out_outer, a.out_inner);
+  // (a quotient, not a product with 1 / D: a constant row's mean is its value, its y is beta)
+  const float width = (float)a.width;
+  for (int64_t row = row0; row < a.rows; row += stride) {
+    float v[NCH][C];
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < NCH; ++i) {
-    const int c = (lane + i * TEAM) * C;
+    for (int i = 0; i < NCH; ++i) {
+      T::widen(next[i], v[i]);
 #pragma unroll
-    for (int j = 0; j < C; ++j) v[i][j] = v[i][j] * rstd * gm[i][j] + bt[i][j];
-    if (c + C <= a.width) vt_store16(y + c, T::pack(v[i]));
-    else if (c < a.width) vt_store_part<T>(y + c, a.width - c, v[i]);
+      for (int j = 0; j < C; ++j) s += v[i][j];
+    }
+    if (row + stride < a.rows)
+      ln_load<T, NCH>(x + vt_row(row + stride, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width,
+                      next);
+    const float mean = ln_team_sum<TEAM>(s, red) / width;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int n = a.width - (lane + i * TEAM) * C;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        v[i][j] -= mean;
+        ss += j < n ? v[i][j] * v[i][j] : 0.f;
+      }
+    }
+    const float var = ln_team_sum<TEAM>(ss, red) / width;
+    const float rstd = 1.f / sqrtf(var + a.epsilon);
+    if (lane == 0 && a.stats != nullptr) {
+      a.stats[2 * row] = mean;
+      a.stats[2 * row + 1] = rstd;
+    }
+    typename T::elem* y = out + vt_row(row, a.inner, a.out_outer, a.out_inner);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+      const int c = (lane + i * TEAM) * C;
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[i][j] = v[i][j] * rstd * gm[i][j] + bt[i][j];
+      if (c + C <= a.width) vt_store16(y + c, T::pack(v[i]));
+      else if (c < a.width) vt_store_part<T>(y + c, a.width - c, v[i]);
+    }
   }
 }
 
@@ -199,27 +208,42 @@ __global__ void __launch_bounds__(TEAM == 64 ? 256 : TEAM)
 aa_layer_norm_bwd_kernel(LnArgs a) {
   constexpr int C = T::C;
   constexpr int PER = TEAM == 64 ? 4 : 1;        // teams of a workgroup
+  // the next row in flight and gamma in registers; 1,024 lanes have 128 registers each and need them
+  // for the sums (spills cost more than reading gamma again)
+  constexpr bool AHEAD = TEAM < 1024;
   __shared__ float red[32];
   __shared__ float sums[(WEIGHTS && TEAM == 64) ? 2 * 64 * NCH * C : 1];
   const int sub = TEAM == 64 ? (threadIdx.x >> 6) : 0;
   const int lane = TEAM == 64 ? (threadIdx.x & 63) : threadIdx.x;
   const float inv = 1.f / (float)a.width;
+  const int64_t row0 = (int64_t)blockIdx.x * PER + sub, stride = (int64_t)gridDim.x * PER;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x);
+  const typename T::elem* dy = reinterpret_cast<const typename T::elem*>(a.dy);
+  uint4 nx[NCH], nd[NCH];          // the next row
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t r) {
+    ln_load<T, NCH>(x + vt_row(r, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, nx);
+    ln_load<T, NCH>(dy + vt_row(r, a.inner, a.dy_outer, a.dy_inner), lane, TEAM, a.width, nd);
+    nmean = a.stats[2 * r];
+    nrstd = a.stats[2 * r + 1];
+  };
+  if (AHEAD && row0 < a.rows) fetch(row0);
   float gm[NCH][C], dg[NCH][C], db[NCH][C];
-  ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
+  if (AHEAD) ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int j = 0; j < C; ++j) dg[i][j] = db[i][j] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * PER + sub; row < a.rows;
-       row += (int64_t)gridDim.x * PER) {
-    const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x) +
-                                vt_row(row, a.inner, a.x_outer, a.x_inner);
-    const typename T::elem* dy = reinterpret_cast<const typename T::elem*>(a.dy) +
-                                 vt_row(row, a.inner, a.dy_outer, a.dy_inner);
+  for (int64_t row = row0; row < a.rows; row += stride) {
+    if (!AHEAD) {
+      fetch(row);
+      ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
+    }
     uint4 qx[NCH], qd[NCH];
-    ln_load<T, NCH>(x, lane, TEAM, a.width, qx);
-    ln_load<T, NCH>(dy, lane, TEAM, a.width, qd);
-    const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) { qx[i] = nx[i]; qd[i] = nd[i]; }
+    const float mean = nmean, rstd = nrstd;
+    if (AHEAD && row + stride < a.rows) fetch(row + stride);
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -381,6 +405,13 @@ static int ln_team(int64_t width) {
   return 0;
 }
 
+// workgroups of the forward pass: enough to fill the machine, several rows each beyond that
+static unsigned ln_fwd_blocks(int64_t rows, int team) {
+  const int64_t teams = team == 64 ? (rows + 3) / 4 : rows;
+  const int64_t most = team <= 256 ? 2048 : team == 512 ? 1024 : 512;
+  return (unsigned)(teams < most ? teams : most);
+}
+
 // workgroups of the backward pass = partials of the weight gradients
 static int64_t ln_groups(int64_t rows, int64_t width) {
   const int team = ln_team(width);
@@ -413,18 +444,19 @@ static LnArgs ln_args(const aa_layer_norm_desc* d) {
 template <typename T>
 static void ln_launch_fwd(const LnArgs& a, hipStream_t st) {
   constexpr int NCH = LN_PER_LANE / T::C;
-  const dim3 rows = vt_grid(a.rows), quads = vt_grid((a.rows + 3) / 4);
-  switch (ln_team(a.width)) {
+  const int team = ln_team(a.width);
+  const dim3 grid(ln_fwd_blocks(a.rows, team));
+  switch (team) {
     case 64:
       if (a.width <= 64 * LN_PER_LANE / 2)
-        aa_layer_norm_fwd_kernel<T, 64, NCH / 2><<<quads, dim3(256), 0, st>>>(a);
+        aa_layer_norm_fwd_kernel<T, 64, NCH / 2><<<grid, dim3(256), 0, st>>>(a);
       else
-        aa_layer_norm_fwd_kernel<T, 64, NCH><<<quads, dim3(256), 0, st>>>(a);
+        aa_layer_norm_fwd_kernel<T, 64, NCH><<<grid, dim3(256), 0, st>>>(a);
       break;
-    case 256: aa_layer_norm_fwd_kernel<T, 256, NCH><<<rows, dim3(256), 0, st>>>(a); break;
-    case 512: aa_layer_norm_fwd_kernel<T, 512, NCH><<<rows, dim3(512), 0, st>>>(a); break;
-    case 1024: aa_layer_norm_fwd_kernel<T, 1024, NCH><<<rows, dim3(1024), 0, st>>>(a); break;
-    default: aa_layer_norm_fwd_wide_kernel<T><<<rows, dim3(1024), 0, st>>>(a);
+    case 256: aa_layer_norm_fwd_kernel<T, 256, NCH><<<grid, dim3(256), 0, st>>>(a); break;
+    case 512: aa_layer_norm_fwd_kernel<T, 512, NCH><<<grid, dim3(512), 0, st>>>(a); break;
+    case 1024: aa_layer_norm_fwd_kernel<T, 1024, NCH><<<grid, dim3(1024), 0, st>>>(a); break;
+    default: aa_layer_norm_fwd_wide_kernel<T><<<vt_grid(a.rows), dim3(1024), 0, st>>>(a);
   }
 }
 

@@ -116,9 +116,3 @@ static inline dim3 vt_grid(int64_t blocks) {
 __device__ static inline int64_t vt_block() {
   return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
 }
-
-__device__ static inline float vt_wave_sum_all(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
