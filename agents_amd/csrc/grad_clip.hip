@@ -20,6 +20,11 @@
 #define CLIP_PIECES 2048           // workgroups a large list is cut into: 8 per CU
 #define CLIP_JOIN 4096
 #define CLIP_UNROLL 4
+// Clipped tensors of this many bytes are stored past the caches (the memory-side one holds 256 MB), so
+// that they do not push out the gradients that the second pass reads again.  bf16, us a call: 268 MB
+// 148 -> 122, 333 MB 200 -> 167; with an update of the clipped tensors behind it 344 -> 348.  Below it
+// costs whoever reads them next: 134 MB 64 -> 64 alone, 137 -> 171 with the update.
+#define CLIP_PAST_CACHE (256ll << 20)
 #define CLIP_FEW 16
 
 template <int N>
@@ -109,7 +114,7 @@ aa_clip_join_kernel(const double* __restrict__ partial, int64_t count, double* _
 template <typename T, int N>
 __global__ void __launch_bounds__(CLIP_THREADS)
 aa_clip_scale_kernel(ClipList<N> L, const double* __restrict__ partial, int64_t count, double clip,
-                     int each, float* __restrict__ norm) {
+                     int each, int past_cache, float* __restrict__ norm) {
   constexpr int C = T::C, U = CLIP_UNROLL, ROUND = CLIP_THREADS * C;
   __shared__ double red[16];
   // the pieces in the opposite order of the first pass: what it read last is still cached
@@ -142,7 +147,8 @@ aa_clip_scale_kernel(ClipList<N> L, const double* __restrict__ partial, int64_t 
     T::widen(q, v);
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] *= f;
-    vt_store16(o + at, T::pack(v));
+    if (past_cache) vt_store16_nt(o + at, T::pack(v));
+    else vt_store16(o + at, T::pack(v));
   };
   while (full) {
 #pragma unroll
@@ -179,10 +185,11 @@ static int clip_check(const int64_t* n_h, int32_t n_tensors, int32_t dtype) {
 
 template <typename T, int N>
 static void clip_launch(const ClipList<N>& L, unsigned blocks, bool scale, const double* partial,
-                        int64_t count, double clip, int each, float* norm, hipStream_t st) {
+                        int64_t count, double clip, int each, int past_cache, float* norm,
+                        hipStream_t st) {
   if (scale)
-    aa_clip_scale_kernel<T, N><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(L, partial, count, clip,
-                                                                            each, norm);
+    aa_clip_scale_kernel<T, N><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(
+        L, partial, count, clip, each, past_cache, norm);
   else
     aa_clip_sumsq_kernel<T, N><<<dim3(blocks), dim3(CLIP_THREADS), 0, st>>>(
         L, const_cast<double*>(partial));
@@ -192,7 +199,7 @@ struct ClipCall {
   const void* const* src;
   void* const* dst;                // null: the global norm only
   const int64_t* n;
-  int32_t n_tensors, dtype, each;
+  int32_t n_tensors, dtype, each, past_cache;
   int64_t piece, total;            // elements of a piece, pieces of the call
   double clip;
   float* norm;
@@ -224,11 +231,14 @@ static void clip_run(const ClipCall& c, hipStream_t st) {
       else if (c.total > CLIP_JOIN) { sums = c.joined; count = 1; }
       float* nrm = c.each ? c.norm + base : (base == 0 ? c.norm : nullptr);
       if (c.dtype == AA_DT_F32)
-        clip_launch<VtF32, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+        clip_launch<VtF32, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, c.past_cache, nrm,
+                               st);
       else if (c.dtype == AA_DT_BF16)
-        clip_launch<VtBf16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+        clip_launch<VtBf16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, c.past_cache, nrm,
+                               st);
       else
-        clip_launch<VtF16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, nrm, st);
+        clip_launch<VtF16, N>(L, blocks, pass == 1, sums, count, c.clip, c.each, c.past_cache, nrm,
+                               st);
       done += blocks;
     }
     if (pass == 0 && !c.each && (c.dst == nullptr || c.total > CLIP_JOIN))
@@ -260,9 +270,14 @@ int aa_clip_tensors(const void* const* src_h, void* const* dst_h, const int64_t*
       return AA_ERR_INVALID;
   if (workspace == nullptr || workspace_bytes < aa_clip_tensors_workspace_bytes(n_h, n_tensors))
     return AA_ERR_RANGE;
-  ClipCall c = {src_h, dst_h, n_h, n_tensors, dtype, each != 0, clip_piece(n_h, n_tensors), 0, clip,
-                norm, (double*)workspace, (double*)workspace + 1};
-  for (int32_t i = 0; i < n_tensors; ++i) c.total += clip_pieces_of(n_h[i], c.piece);
+  ClipCall c = {src_h, dst_h, n_h, n_tensors, dtype, each != 0, 0, clip_piece(n_h, n_tensors), 0,
+                clip, norm, (double*)workspace, (double*)workspace + 1};
+  int64_t elements = 0;
+  for (int32_t i = 0; i < n_tensors; ++i) {
+    c.total += clip_pieces_of(n_h[i], c.piece);
+    elements += n_h[i];
+  }
+  c.past_cache = elements * (dtype == AA_DT_F32 ? 4 : 2) >= CLIP_PAST_CACHE;
   if (c.total > 0x7fffff) return AA_ERR_RANGE;
   // the arguments of a launch are written by the host for every call: a short list for few tensors
   if (n_tensors <= CLIP_FEW) clip_run<CLIP_FEW>(c, (hipStream_t)stream);

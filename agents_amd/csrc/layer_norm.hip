@@ -3,21 +3,25 @@
 //   y = h gamma + beta
 //   g = dy gamma;  dx = rstd (g - mean(g) - h mean(g h)) * act'(x);  dgamma = sum_rows dy h;
 //   dbeta = sum_rows dy
-// Everything is held in fp32; x, dy, y and dx are rounded once on their way to memory.  Bound by HBM:
-// a row is read once into registers by one team (a wave up to 1,024 columns, a workgroup of
-// 256 / 512 / 1,024 lanes beyond), the mean and the squares about it come from the registers, so the
-// variance has no cancellation and the row is not read a second time.  The weight gradients need every
-// row: a team walks many rows with its columns' sums in registers and leaves one partial per
-// workgroup, a second launch adds the partials in a fixed order (no atomics: same bits every call).
-// Rows wider than 16,384 columns do not fit the registers beside these sums and take loops.
+// Everything is held in fp32; x, dy, y and dx are rounded once on their way to memory.  Bound by HBM: a
+// row is read once into registers by one team of lanes -- 8 for up to 64 columns, a workgroup for
+// thousands --, the mean and the squares about it come from the registers, so the variance has no
+// cancellation and the row is not read a second time; a team's next row is in flight meanwhile.
+// The weight gradients need every row: a team walks many rows with its columns' sums in registers, the
+// teams of a workgroup add theirs in LDS, and a second launch adds the workgroups' partials, all in a
+// fixed order (no atomics: same bits every call).  One workgroup of 1,024 lanes per CU: the partials
+// cost a write and a read of 8 bytes a column and workgroup, which at 512 workgroups of 256 lanes was
+// as much as the rows themselves for 2000 rows of 2048.
+// Rows past 8,192 columns have no registers left for the weights' sums: their columns are summed by a
+// pass of its own; past 16,384 the rows are walked in loops.
 #include <math.h>
 #include "common.h"
 #include "agents_amd.h"
 #include "vec_types.h"
 #include "wave_ops.h"
 
-#define LN_MAX_WIDTH_REG 16384
-#define LN_PER_LANE 16
+#define LN_FWD_COLUMNS 16384       // columns that a workgroup's registers hold
+#define LN_BWD_COLUMNS 8192        // the same beside the weights' sums
 
 struct LnArgs {
   int64_t rows, inner;
@@ -33,36 +37,41 @@ struct LnArgs {
   int mask_act;
 };
 
-template <int TEAM>
-__device__ static inline float ln_team_sum(float v, float* red) {
-  v = wv_sum(v);
-  if constexpr (TEAM == 64) return v;
-  constexpr int NW = TEAM / 64;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0.f;
+// Sums over a team of TEAM lanes in every one of them.  Teams past a wave meet in `red`, each call in
+// a half of its own (`turn` alternates): one barrier.  TEAMS teams of a workgroup call in step.
+template <int TEAM, int TEAMS>
+__device__ static inline void ln_team_sum2(float& a, float& b, float (*red)[2][16], int& turn) {
+  a = wv_group_sum<(TEAM < 64 ? TEAM : 64)>(a);
+  b = wv_group_sum<(TEAM < 64 ? TEAM : 64)>(b);
+  if constexpr (TEAM > 64) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      red[turn][0][wave] = a;
+      red[turn][1][wave] = b;
+    }
+    __syncthreads();
+    const int w0 = TEAMS == 1 ? 0 : wave & ~(TEAM / 64 - 1);
+    a = b = 0.f;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) s += red[w];
-  return s;
-}
-
-// two sums behind one pair of barriers
-template <int TEAM>
-__device__ static inline void ln_team_sum2(float& a, float& b, float* red) {
-  a = wv_sum(a);
-  b = wv_sum(b);
-  if constexpr (TEAM == 64) return;
-  constexpr int NW = TEAM / 64;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[threadIdx.x >> 6] = a;
-    red[NW + (threadIdx.x >> 6)] = b;
+    for (int w = 0; w < TEAM / 64; ++w) {
+      a += red[turn][0][w0 + w];
+      b += red[turn][1][w0 + w];
+    }
+    turn ^= 1;
   }
-  __syncthreads();
-  a = b = 0.f;
+}
+template <int TEAM>
+__device__ static inline float ln_team_sum(float v, float (*red)[2][16], int& turn) {
+  v = wv_group_sum<(TEAM < 64 ? TEAM : 64)>(v);
+  if constexpr (TEAM > 64) {       // (one team: the workgroup)
+    if ((threadIdx.x & 63) == 0) red[turn][0][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) { a += red[w]; b += red[NW + w]; }
+    for (int w = 0; w < TEAM / 64; ++w) v += red[turn][0][w];
+    turn ^= 1;
+  }
+  return v;
 }
 
 template <typename T, int NCH>
@@ -107,25 +116,34 @@ __device__ static inline void ln_load_weight(const float* w, int lane, int team,
 // A team walks rows `stride` apart: the weights are read once, the next row's loads are in flight while
 // this one is worked on.
 template <typename T, int TEAM, int NCH>
-__global__ void __launch_bounds__(TEAM == 64 ? 256 : TEAM)
+__global__ void __launch_bounds__(TEAM <= 256 ? 256 : TEAM)
 aa_layer_norm_fwd_kernel(LnArgs a) {
   constexpr int C = T::C;
-  constexpr int PER = TEAM == 64 ? 4 : 1;        // teams of a workgroup
-  __shared__ float red[32];
-  const int64_t row0 = (int64_t)blockIdx.x * PER + (TEAM == 64 ? threadIdx.x >> 6 : 0);
+  constexpr int PER = TEAM <= 256 ? 256 / TEAM : 1;        // teams of a workgroup
+  static_assert(TEAM <= 64 || PER == 1, "teams that meet a barrier fill the workgroup");
+  __shared__ float red[2][2][16];
+  int turn = 0;
   const int64_t stride = (int64_t)gridDim.x * PER;
-  const int lane = TEAM == 64 ? (threadIdx.x & 63) : threadIdx.x;
-  if (row0 >= a.rows) return;      // (the whole workgroup, or a wave that meets no barrier)
+  const int lane = threadIdx.x % TEAM;
+  // Teams of one wave stay in step: those past the last row work on it once more, their loop ends
+  // with the wave's and they store nothing.
+  const int64_t wave0 = (int64_t)blockIdx.x * PER + (TEAM < 64 ? (threadIdx.x & ~63u) / TEAM
+                                                               : threadIdx.x / TEAM);
+  const int ahead = TEAM < 64 ? (int)(threadIdx.x & 63u) / TEAM : 0;
+  if (wave0 >= a.rows) return;     // (the whole workgroup, or a wave that meets no barrier)
+  const int64_t last = a.rows - 1;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x);
   typename T::elem* out = reinterpret_cast<typename T::elem*>(a.out);
   uint4 next[NCH];
+  const int64_t row0 = wave0 + ahead < last ? wave0 + ahead : last;
   ln_load<T, NCH>(x + vt_row(row0, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, next);
   float gm[NCH][C], bt[NCH][C];
   ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
   ln_load_weight<C, NCH>(a.beta, lane, TEAM, a.width, 0.f, bt);
   // (a quotient, not a product with 1 / D: a constant row's mean is its value, its y is beta)
   const float width = (float)a.width;
-  for (int64_t row = row0; row < a.rows; row += stride) {
+  for (int64_t base = wave0; base < a.rows; base += stride) {
+    const int64_t row = base + ahead;
     float v[NCH][C];
     float s = 0.f;
 #pragma unroll
@@ -134,10 +152,11 @@ aa_layer_norm_fwd_kernel(LnArgs a) {
 #pragma unroll
       for (int j = 0; j < C; ++j) s += v[i][j];
     }
-    if (row + stride < a.rows)
-      ln_load<T, NCH>(x + vt_row(row + stride, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width,
-                      next);
-    const float mean = ln_team_sum<TEAM>(s, red) / width;
+    if (base + stride < a.rows) {
+      const int64_t r = row + stride < last ? row + stride : last;
+      ln_load<T, NCH>(x + vt_row(r, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, next);
+    }
+    const float mean = ln_team_sum<TEAM>(s, red, turn) / width;
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -148,8 +167,9 @@ aa_layer_norm_fwd_kernel(LnArgs a) {
         ss += j < n ? v[i][j] * v[i][j] : 0.f;
       }
     }
-    const float var = ln_team_sum<TEAM>(ss, red) / width;
+    const float var = ln_team_sum<TEAM>(ss, red, turn) / width;
     const float rstd = 1.f / sqrtf(var + a.epsilon);
+    if (row > last) continue;
     if (lane == 0 && a.stats != nullptr) {
       a.stats[2 * row] = mean;
       a.stats[2 * row + 1] = rstd;
@@ -166,10 +186,24 @@ aa_layer_norm_fwd_kernel(LnArgs a) {
   }
 }
 
+// one chunk of a row as fp32 (0 past its end)
+template <typename T>
+__device__ static inline void ln_chunk(const typename T::elem* x, int c, int width, float (&v)[T::C]) {
+  if (c + T::C <= width) T::widen(vt_load16(x + c), v);
+  else vt_load_part<T>(x + c, width - c, 0.f, v);
+}
+template <typename T>
+__device__ static inline void ln_put(typename T::elem* y, int c, int width, const float (&v)[T::C]) {
+  if (c + T::C <= width) vt_store16(y + c, T::pack(v));
+  else vt_store_part<T>(y + c, width - c, v);
+}
+
 // rows wider than the registers hold: a workgroup per row, three passes
 template <typename T>
 __global__ void __launch_bounds__(1024) aa_layer_norm_fwd_wide_kernel(LnArgs a) {
-  __shared__ float red[32];
+  constexpr int C = T::C;
+  __shared__ float red[2][2][16];
+  int turn = 0;
   const int64_t row = vt_block();
   if (row >= a.rows) return;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x) +
@@ -178,22 +212,33 @@ __global__ void __launch_bounds__(1024) aa_layer_norm_fwd_wide_kernel(LnArgs a) 
                         vt_row(row, a.inner, a.out_outer, a.out_inner);
   const float width = (float)a.width;
   float s = 0.f;
-  for (int c = threadIdx.x; c < a.width; c += 1024) s += T::one(x[c]);
-  const float mean = ln_team_sum<1024>(s, red) / width;
-  float ss = 0.f;
-  for (int c = threadIdx.x; c < a.width; c += 1024) {
-    const float d = T::one(x[c]) - mean;
-    ss += d * d;
+  for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
+    float v[C];
+    ln_chunk<T>(x, c, a.width, v);
+#pragma unroll
+    for (int j = 0; j < C; ++j) s += v[j];
   }
-  const float rstd = 1.f / sqrtf(ln_team_sum<1024>(ss, red) / width + a.epsilon);
+  const float mean = ln_team_sum<1024>(s, red, turn) / width;
+  float ss = 0.f;
+  for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
+    float v[C];
+    ln_chunk<T>(x, c, a.width, v);
+#pragma unroll
+    for (int j = 0; j < C; ++j) ss += c + j < a.width ? (v[j] - mean) * (v[j] - mean) : 0.f;
+  }
+  const float rstd = 1.f / sqrtf(ln_team_sum<1024>(ss, red, turn) / width + a.epsilon);
   if (threadIdx.x == 0 && a.stats != nullptr) {
     a.stats[2 * row] = mean;
     a.stats[2 * row + 1] = rstd;
   }
-  for (int c = threadIdx.x; c < a.width; c += 1024) {
-    const float g = a.gamma != nullptr ? a.gamma[c] : 1.f;
-    const float b = a.beta != nullptr ? a.beta[c] : 0.f;
-    y[c] = T::put((T::one(x[c]) - mean) * rstd * g + b);
+  for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
+    float v[C], gm[1][C], bt[1][C];
+    ln_chunk<T>(x, c, a.width, v);
+    ln_load_weight<C, 1>(a.gamma, c / C, 0, a.width, 1.f, gm);
+    ln_load_weight<C, 1>(a.beta, c / C, 0, a.width, 0.f, bt);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = (v[j] - mean) * rstd * gm[0][j] + bt[0][j];
+    ln_put<T>(y, c, a.width, v);
   }
 }
 
@@ -203,38 +248,46 @@ __device__ static inline float ln_act_grad(float y, int kind) {
   return 1.f;
 }
 
+// Workgroups of 1,024 lanes = PER teams, each a row at a time.
 template <typename T, int TEAM, int NCH, bool WEIGHTS>
-__global__ void __launch_bounds__(TEAM == 64 ? 256 : TEAM)
-aa_layer_norm_bwd_kernel(LnArgs a) {
+__global__ void __launch_bounds__(1024) aa_layer_norm_bwd_kernel(LnArgs a) {
   constexpr int C = T::C;
-  constexpr int PER = TEAM == 64 ? 4 : 1;        // teams of a workgroup
-  // the next row in flight and gamma in registers; 1,024 lanes have 128 registers each and need them
-  // for the sums (spills cost more than reading gamma again)
-  constexpr bool AHEAD = TEAM < 1024;
-  __shared__ float red[32];
-  __shared__ float sums[(WEIGHTS && TEAM == 64) ? 2 * 64 * NCH * C : 1];
-  const int sub = TEAM == 64 ? (threadIdx.x >> 6) : 0;
-  const int lane = TEAM == 64 ? (threadIdx.x & 63) : threadIdx.x;
+  constexpr int PER = 1024 / TEAM;
+  // gamma and the next row in registers: 128 registers a lane hold them beside the sums of 8 columns
+  constexpr bool AHEAD = NCH * C <= 8;
+  constexpr int COLS = TEAM * NCH * C;           // columns of a team
+  constexpr int UNIT = TEAM < 64 ? 64 : TEAM;    // lanes that hold one set of sums at the end
+  constexpr int UNITS = 1024 / UNIT;
+  __shared__ float red[2][2][16];
+  __shared__ float sums[WEIGHTS && UNITS > 1 ? UNITS / 2 : 1][2][WEIGHTS && UNITS > 1 ? COLS : 1];
+  int turn = 0;
+  const int sub = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
   const float inv = 1.f / (float)a.width;
-  const int64_t row0 = (int64_t)blockIdx.x * PER + sub, stride = (int64_t)gridDim.x * PER;
+  const int64_t row0 = (int64_t)blockIdx.x * PER, stride = (int64_t)gridDim.x * PER;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x);
   const typename T::elem* dy = reinterpret_cast<const typename T::elem*>(a.dy);
-  uint4 nx[NCH], nd[NCH];          // the next row
-  float nmean = 0.f, nrstd = 0.f;
+  uint4 nx[NCH], nd[NCH];          // the next row; zeros past the last one, which add nothing
+  float nmean, nrstd;
   auto fetch = [&](int64_t r) {
-    ln_load<T, NCH>(x + vt_row(r, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, nx);
-    ln_load<T, NCH>(dy + vt_row(r, a.inner, a.dy_outer, a.dy_inner), lane, TEAM, a.width, nd);
-    nmean = a.stats[2 * r];
-    nrstd = a.stats[2 * r + 1];
+    nmean = nrstd = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) nx[i] = nd[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (r < a.rows) {
+      ln_load<T, NCH>(x + vt_row(r, a.inner, a.x_outer, a.x_inner), lane, TEAM, a.width, nx);
+      ln_load<T, NCH>(dy + vt_row(r, a.inner, a.dy_outer, a.dy_inner), lane, TEAM, a.width, nd);
+      nmean = a.stats[2 * r];
+      nrstd = a.stats[2 * r + 1];
+    }
   };
-  if (AHEAD && row0 < a.rows) fetch(row0);
+  if (AHEAD) fetch(row0 + sub);
   float gm[NCH][C], dg[NCH][C], db[NCH][C];
   if (AHEAD) ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
 #pragma unroll
   for (int i = 0; i < NCH; ++i)
 #pragma unroll
     for (int j = 0; j < C; ++j) dg[i][j] = db[i][j] = 0.f;
-  for (int64_t row = row0; row < a.rows; row += stride) {
+  for (int64_t base = row0; base < a.rows; base += stride) {       // (workgroup-uniform)
+    const int64_t row = base + sub;
     if (!AHEAD) {
       fetch(row);
       ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
@@ -243,7 +296,7 @@ aa_layer_norm_bwd_kernel(LnArgs a) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) { qx[i] = nx[i]; qd[i] = nd[i]; }
     const float mean = nmean, rstd = nrstd;
-    if (AHEAD && row + stride < a.rows) fetch(row + stride);
+    if (AHEAD && base + stride < a.rows) fetch(row + stride);
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -262,10 +315,10 @@ aa_layer_norm_bwd_kernel(LnArgs a) {
         }
       }
     }
-    ln_team_sum2<TEAM>(c1, c2, red);
+    ln_team_sum2<TEAM, PER>(c1, c2, red, turn);
     c1 *= inv;
     c2 *= inv;
-    if (a.out != nullptr) {
+    if (a.out != nullptr && row < a.rows) {
       typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.out) +
                              vt_row(row, a.inner, a.out_outer, a.out_inner);
 #pragma unroll
@@ -280,34 +333,57 @@ aa_layer_norm_bwd_kernel(LnArgs a) {
           r[j] = rstd * (dv[j] * gm[i][j] - c1 - h * c2);
           if (a.mask_act != AA_ACT_NONE) r[j] *= ln_act_grad(xv[j], a.mask_act);
         }
-        if (c + C <= a.width) vt_store16(dx + c, T::pack(r));
-        else if (c < a.width) vt_store_part<T>(dx + c, a.width - c, r);
+        if (c < a.width) ln_put<T>(dx, c, a.width, r);
       }
     }
   }
   if constexpr (WEIGHTS) {
-    float* out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
-    if constexpr (TEAM == 64) {
-      // the four waves' sums, added in the order of the waves
-      for (int w = 0; w < 4; ++w) {
-        if (sub == w) {
+    // teams of a wave, then the units of the workgroup in halves
+    if constexpr (TEAM < 64) {
 #pragma unroll
-          for (int i = 0; i < NCH; ++i)
+      for (int i = 0; i < NCH; ++i)
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-              const int at = (lane + i * 64) * C + j;
-              const int at2 = at + 64 * NCH * C;
-              sums[at] = w == 0 ? dg[i][j] : sums[at] + dg[i][j];
-              sums[at2] = w == 0 ? db[i][j] : sums[at2] + db[i][j];
-            }
+        for (int j = 0; j < C; ++j) {
+          const auto add = [](float p, float q) { return p + q; };
+          if constexpr (TEAM <= 8) {      // (lane ^ 8: a row rotated by half of it)
+            dg[i][j] += __uint_as_float(wv_xor<8>(__float_as_uint(dg[i][j]), 0));
+            db[i][j] += __uint_as_float(wv_xor<8>(__float_as_uint(db[i][j]), 0));
+          }
+          if constexpr (TEAM <= 16) {
+            dg[i][j] = wv_step<16>(dg[i][j], add);
+            db[i][j] = wv_step<16>(db[i][j], add);
+          }
+          dg[i][j] = wv_step<32>(dg[i][j], add);
+          db[i][j] = wv_step<32>(db[i][j], add);
         }
-        __syncthreads();
+    }
+    const int unit = threadIdx.x / UNIT;
+    const bool speaks = TEAM >= 64 || (threadIdx.x & 63) < TEAM;
+#pragma unroll
+    for (int half = UNITS / 2; half >= 1; half >>= 1) {
+      if (unit >= half && unit < 2 * half && speaks) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            sums[unit - half][0][(lane + i * TEAM) * C + j] = dg[i][j];
+            sums[unit - half][1][(lane + i * TEAM) * C + j] = db[i][j];
+          }
       }
-      for (int c = threadIdx.x; c < a.width; c += 256) {
-        out[c] = sums[c];
-        out[a.width + c] = sums[64 * NCH * C + c];
+      __syncthreads();
+      if (unit < half && speaks) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            dg[i][j] += sums[unit][0][(lane + i * TEAM) * C + j];
+            db[i][j] += sums[unit][1][(lane + i * TEAM) * C + j];
+          }
       }
-    } else {
+      __syncthreads();
+    }
+    if (unit == 0 && speaks) {
+      float* out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
 #pragma unroll
@@ -324,7 +400,9 @@ aa_layer_norm_bwd_kernel(LnArgs a) {
 
 template <typename T>
 __global__ void __launch_bounds__(1024) aa_layer_norm_dx_wide_kernel(LnArgs a) {
-  __shared__ float red[32];
+  constexpr int C = T::C;
+  __shared__ float red[2][2][16];
+  int turn = 0;
   const int64_t row = vt_block();
   if (row >= a.rows) return;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x) +
@@ -336,40 +414,78 @@ __global__ void __launch_bounds__(1024) aa_layer_norm_dx_wide_kernel(LnArgs a) {
   const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
   const float inv = 1.f / (float)a.width;
   float c1 = 0.f, c2 = 0.f;
-  for (int c = threadIdx.x; c < a.width; c += 1024) {
-    const float g = T::one(dy[c]) * (a.gamma != nullptr ? a.gamma[c] : 1.f);
-    c1 += g;
-    c2 += g * ((T::one(x[c]) - mean) * rstd);
+  for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
+    float xv[C], dv[C], gm[1][C];
+    ln_chunk<T>(x, c, a.width, xv);
+    ln_chunk<T>(dy, c, a.width, dv);
+    ln_load_weight<C, 1>(a.gamma, c / C, 0, a.width, 1.f, gm);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const float g = dv[j] * gm[0][j];
+      c1 += g;
+      c2 += g * ((xv[j] - mean) * rstd);
+    }
   }
-  ln_team_sum2<1024>(c1, c2, red);
+  ln_team_sum2<1024, 1>(c1, c2, red, turn);
   c1 *= inv;
   c2 *= inv;
-  for (int c = threadIdx.x; c < a.width; c += 1024) {
-    const float xv = T::one(x[c]), h = (xv - mean) * rstd;
-    const float g = T::one(dy[c]) * (a.gamma != nullptr ? a.gamma[c] : 1.f);
-    float r = rstd * (g - c1 - h * c2);
-    if (a.mask_act != AA_ACT_NONE) r *= ln_act_grad(xv, a.mask_act);
-    dx[c] = T::put(r);
+  for (int c = threadIdx.x * C; c < a.width; c += 1024 * C) {
+    float xv[C], dv[C], gm[1][C];
+    ln_chunk<T>(x, c, a.width, xv);
+    ln_chunk<T>(dy, c, a.width, dv);
+    ln_load_weight<C, 1>(a.gamma, c / C, 0, a.width, 1.f, gm);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const float h = (xv[j] - mean) * rstd;
+      dv[j] = rstd * (dv[j] * gm[0][j] - c1 - h * c2);
+      if (a.mask_act != AA_ACT_NONE) dv[j] *= ln_act_grad(xv[j], a.mask_act);
+    }
+    ln_put<T>(dx, c, a.width, dv);
   }
 }
 
-// weight gradients of wide rows: a lane owns a column, grid = (column blocks, row groups)
+// weight gradients of wide rows: a lane owns a chunk of columns, grid = (column blocks, row groups)
 template <typename T>
 __global__ void __launch_bounds__(256) aa_layer_norm_dw_wide_kernel(LnArgs a) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  constexpr int C = T::C, U = 4;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * C;
   if (c >= a.width) return;
-  float dg = 0.f, db = 0.f;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float xv = T::one(reinterpret_cast<const typename T::elem*>(
-        a.x)[vt_row(row, a.inner, a.x_outer, a.x_inner) + c]);
-    const float dv = T::one(reinterpret_cast<const typename T::elem*>(
-        a.dy)[vt_row(row, a.inner, a.dy_outer, a.dy_inner) + c]);
-    dg += dv * ((xv - a.stats[2 * row]) * a.stats[2 * row + 1]);
-    db += dv;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.x) + c;
+  const typename T::elem* dy = reinterpret_cast<const typename T::elem*>(a.dy) + c;
+  float dg[C], db[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) dg[j] = db[j] = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += (int64_t)U * gridDim.y) {
+    float xv[U][C], dv[U][C];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = row + (int64_t)u * gridDim.y;
+#pragma unroll
+      for (int j = 0; j < C; ++j) xv[u][j] = dv[u][j] = 0.f;
+      if (r < a.rows) {
+        ln_chunk<T>(x + vt_row(r, a.inner, a.x_outer, a.x_inner), 0, a.width - c, xv[u]);
+        ln_chunk<T>(dy + vt_row(r, a.inner, a.dy_outer, a.dy_inner), 0, a.width - c, dv[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = row + (int64_t)u * gridDim.y;
+      if (r >= a.rows) break;
+      const float mean = a.stats[2 * r], rstd = a.stats[2 * r + 1];
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        dg[j] += dv[u][j] * ((xv[u][j] - mean) * rstd);
+        db[j] += dv[u][j];
+      }
+    }
   }
   float* out = a.partial + (int64_t)blockIdx.y * 2 * a.width;
-  out[c] = dg;
-  out[a.width + c] = db;
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+    if (c + j < a.width) {
+      out[c + j] = dg[j];
+      out[a.width + c + j] = db[j];
+    }
 }
 
 // sums of the partials' columns: 32 columns x 32 lanes along the partials per workgroup
@@ -380,8 +496,23 @@ aa_layer_norm_join_kernel(const float* __restrict__ partial, int groups, int wid
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   float s = 0.f;
-  if (c < 2 * width)
-    for (int p = ty; p < groups; p += 32) s += partial[(int64_t)p * 2 * width + c];
+  if (c < 2 * width) {
+    const float* q = partial + c;
+    int p = ty;
+    for (; p + 7 * 32 < groups; p += 8 * 32) {       // (eight loads in flight)
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = q[(int64_t)(p + 32 * i) * 2 * width];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = p + 32 * i < groups ? q[(int64_t)(p + 32 * i) * 2 * width] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += v[i];
+  }
   red[ty][tx] = s;
   __syncthreads();
   if (ty == 0 && c < 2 * width) {
@@ -396,29 +527,40 @@ aa_layer_norm_join_kernel(const float* __restrict__ partial, int groups, int wid
   }
 }
 
-// lanes of a row's team (0: the loops)
-static int ln_team(int64_t width) {
-  if (width <= 64 * LN_PER_LANE) return 64;
-  if (width <= 256 * LN_PER_LANE) return 256;
-  if (width <= 512 * LN_PER_LANE) return 512;
-  if (width <= LN_MAX_WIDTH_REG) return 1024;
-  return 0;
+// lanes of a row's team, forward (0: the loops)
+static int ln_fwd_team(int64_t width) {
+  if (width <= 64) return 8;
+  if (width <= 256) return 32;
+  if (width <= 1024) return 64;
+  if (width <= 4096) return 256;
+  if (width <= 8192) return 512;
+  return width <= LN_FWD_COLUMNS ? 1024 : 0;
 }
 
 // workgroups of the forward pass: enough to fill the machine, several rows each beyond that
 static unsigned ln_fwd_blocks(int64_t rows, int team) {
-  const int64_t teams = team == 64 ? (rows + 3) / 4 : rows;
+  const int per = team <= 256 ? 256 / team : 1;
+  const int64_t teams = (rows + per - 1) / per;
   const int64_t most = team <= 256 ? 2048 : team == 512 ? 1024 : 512;
   return (unsigned)(teams < most ? teams : most);
 }
 
-// workgroups of the backward pass = partials of the weight gradients
+// lanes of a row's team, backward: 8 columns each (0: two passes)
+static int ln_bwd_team(int64_t width) {
+  if (width > LN_BWD_COLUMNS) return 0;
+  int team = 8;
+  while (team * 8 < width) team *= team == 8 ? 4 : 2;
+  return team;
+}
+
+// workgroups of the backward pass = partials of the weight gradients: one per CU at most, and no more
+// than share the rounds evenly
 static int64_t ln_groups(int64_t rows, int64_t width) {
-  const int team = ln_team(width);
+  const int team = ln_bwd_team(width);
   if (team == 0) return rows < 64 ? rows : 64;
-  const int64_t teams = team == 64 ? (rows + 3) / 4 : rows;
-  const int64_t most = team == 64 ? 1024 : team == 256 ? 512 : 256;
-  return teams < most ? teams : most;
+  const int64_t sets = (rows + 1024 / team - 1) / (1024 / team);
+  const int64_t rounds = (sets + 255) / 256;
+  return (sets + rounds - 1) / rounds;
 }
 
 static int ln_check(const aa_layer_norm_desc* d) {
@@ -443,49 +585,47 @@ static LnArgs ln_args(const aa_layer_norm_desc* d) {
 
 template <typename T>
 static void ln_launch_fwd(const LnArgs& a, hipStream_t st) {
-  constexpr int NCH = LN_PER_LANE / T::C;
-  const int team = ln_team(a.width);
-  const dim3 grid(ln_fwd_blocks(a.rows, team));
+  constexpr int N8 = 8 / T::C, N16 = 16 / T::C;       // chunks of a lane
+  const int team = ln_fwd_team(a.width);
+  const dim3 grid(team != 0 ? ln_fwd_blocks(a.rows, team) : 1);
   switch (team) {
+    case 8: aa_layer_norm_fwd_kernel<T, 8, N8><<<grid, dim3(256), 0, st>>>(a); break;
+    case 32: aa_layer_norm_fwd_kernel<T, 32, N8><<<grid, dim3(256), 0, st>>>(a); break;
     case 64:
-      if (a.width <= 64 * LN_PER_LANE / 2)
-        aa_layer_norm_fwd_kernel<T, 64, NCH / 2><<<grid, dim3(256), 0, st>>>(a);
-      else
-        aa_layer_norm_fwd_kernel<T, 64, NCH><<<grid, dim3(256), 0, st>>>(a);
+      if (a.width <= 512) aa_layer_norm_fwd_kernel<T, 64, N8><<<grid, dim3(256), 0, st>>>(a);
+      else aa_layer_norm_fwd_kernel<T, 64, N16><<<grid, dim3(256), 0, st>>>(a);
       break;
-    case 256: aa_layer_norm_fwd_kernel<T, 256, NCH><<<grid, dim3(256), 0, st>>>(a); break;
-    case 512: aa_layer_norm_fwd_kernel<T, 512, NCH><<<grid, dim3(512), 0, st>>>(a); break;
-    case 1024: aa_layer_norm_fwd_kernel<T, 1024, NCH><<<grid, dim3(1024), 0, st>>>(a); break;
+    case 256: aa_layer_norm_fwd_kernel<T, 256, N16><<<grid, dim3(256), 0, st>>>(a); break;
+    case 512: aa_layer_norm_fwd_kernel<T, 512, N16><<<grid, dim3(512), 0, st>>>(a); break;
+    case 1024: aa_layer_norm_fwd_kernel<T, 1024, N16><<<grid, dim3(1024), 0, st>>>(a); break;
     default: aa_layer_norm_fwd_wide_kernel<T><<<vt_grid(a.rows), dim3(1024), 0, st>>>(a);
   }
 }
 
 template <typename T, bool WEIGHTS>
 static void ln_launch_bwd(const LnArgs& a, unsigned groups, hipStream_t st) {
-  constexpr int NCH = LN_PER_LANE / T::C;
-  switch (ln_team(a.width)) {
-    case 64:
-      if (a.width <= 64 * LN_PER_LANE / 2)
-        aa_layer_norm_bwd_kernel<T, 64, NCH / 2, WEIGHTS><<<dim3(groups), dim3(256), 0, st>>>(a);
-      else
-        aa_layer_norm_bwd_kernel<T, 64, NCH, WEIGHTS><<<dim3(groups), dim3(256), 0, st>>>(a);
-      break;
-    case 256:
-      aa_layer_norm_bwd_kernel<T, 256, NCH, WEIGHTS><<<dim3(groups), dim3(256), 0, st>>>(a);
-      break;
-    case 512:
-      aa_layer_norm_bwd_kernel<T, 512, NCH, WEIGHTS><<<dim3(groups), dim3(512), 0, st>>>(a);
-      break;
-    case 1024:
-      aa_layer_norm_bwd_kernel<T, 1024, NCH, WEIGHTS><<<dim3(groups), dim3(1024), 0, st>>>(a);
-      break;
+  constexpr int N8 = 8 / T::C, N16 = 16 / T::C;
+  const dim3 grid(groups), block(1024);
+  switch (ln_bwd_team(a.width)) {
+    case 8: aa_layer_norm_bwd_kernel<T, 8, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 32: aa_layer_norm_bwd_kernel<T, 32, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 64: aa_layer_norm_bwd_kernel<T, 64, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 128: aa_layer_norm_bwd_kernel<T, 128, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 256: aa_layer_norm_bwd_kernel<T, 256, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 512: aa_layer_norm_bwd_kernel<T, 512, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
+    case 1024: aa_layer_norm_bwd_kernel<T, 1024, N8, WEIGHTS><<<grid, block, 0, st>>>(a); break;
     default:
       // (the weights first: dx may be stored over x or dy)
-      if (WEIGHTS)
-        aa_layer_norm_dw_wide_kernel<T><<<dim3((unsigned)((a.width + 255) / 256), groups),
-                                          dim3(256), 0, st>>>(a);
-      if (a.out != nullptr)
-        aa_layer_norm_dx_wide_kernel<T><<<vt_grid(a.rows), dim3(1024), 0, st>>>(a);
+      if (WEIGHTS) {
+        const unsigned blocks = (unsigned)((a.width + 256 * T::C - 1) / (256 * T::C));
+        aa_layer_norm_dw_wide_kernel<T><<<dim3(blocks, groups), dim3(256), 0, st>>>(a);
+      }
+      if (a.out == nullptr) break;
+      if (a.width <= LN_FWD_COLUMNS)
+        aa_layer_norm_bwd_kernel<T, 1024, N16, false>
+            <<<dim3((unsigned)(a.rows < 512 ? a.rows : 512)), block, 0, st>>>(a);
+      else
+        aa_layer_norm_dx_wide_kernel<T><<<vt_grid(a.rows), block, 0, st>>>(a);
   }
 }
 

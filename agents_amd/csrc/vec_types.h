@@ -82,6 +82,13 @@ __device__ static inline uint4 vt_load16(const void* p) {
 }
 __device__ static inline void vt_store16(void* p, const uint4& q) { __builtin_memcpy(p, &q, 16); }
 
+typedef unsigned vt_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+// (streaming: the lines are the first that the caches give up)
+__device__ static inline void vt_store16_nt(void* p, const uint4& q) {
+  const vt_u32x4 v = {q.x, q.y, q.z, q.w};
+  __builtin_nontemporal_store(v, reinterpret_cast<vt_u32x4*>(p));
+}
+
 // chunk of which only the first `n` elements exist (n <= 0: none); the others read as `fill`
 template <typename T>
 __device__ static inline void vt_load_part(const typename T::elem* p, int n, float fill,
