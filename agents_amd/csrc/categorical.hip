@@ -22,6 +22,7 @@
 #define CAT_LOWEST (-3.402823466e+38f)
 #define CAT_LOG2E 1.4426950408889634f
 #define CAT_LN2 0.6931471805599453f
+#define CAT_FEW 8                  // elements a lane holds of a row of few actions (up to 64 x 8)
 #define CAT_WAVE_VOCAB 4096        // up to here a wave takes a row, beyond a workgroup
 #define CAT_SPLIT_BLOCKS 1024      // workgroups that fill the machine
 // A gradient of this many bytes is stored past the caches: with the logits it exceeds the 256 MB of the
@@ -148,12 +149,11 @@ __device__ static inline void cat_top_offer(CatTop& t, float v, int index, bool 
 }
 
 // ---- the row's end: log_prob, entropy, stats, alternatives -----------------------------------------
-template <typename T, int MB>
-__device__ static inline bool cat_allowed(const CatArgs& a, int64_t row, int64_t v) {
-  if (MB == 0) return true;
-  const int64_t at = vt_row(row, a.inner, a.k_outer, a.k_inner) + v;
-  return MB == 1 ? reinterpret_cast<const uint8_t*>(a.mask)[at] != 0
-                 : reinterpret_cast<const int32_t*>(a.mask)[at] != 0;
+template <int MB>
+__device__ static inline bool cat_allowed(const void* mask, int64_t at) {
+  if (MB == 1) return reinterpret_cast<const uint8_t*>(mask)[at] != 0;
+  if (MB == 4) return reinterpret_cast<const int32_t*>(mask)[at] != 0;
+  return true;
 }
 
 __device__ static inline int64_t cat_action(const CatArgs& a, int64_t row) {
@@ -164,11 +164,21 @@ __device__ static inline int64_t cat_action(const CatArgs& a, int64_t row) {
   return v - a.first_action;
 }
 
+// the action's logit, -inf where it is masked (read before the row, so that nothing waits for it)
+template <typename T, int MB>
+__device__ static inline float cat_action_logit(const CatArgs& a, int64_t row, int64_t action) {
+  if (action < 0 || action >= a.vocab) return 0.f;
+  const float x = T::one(reinterpret_cast<const typename T::elem*>(
+      a.logits)[vt_row(row, a.inner, a.x_outer, a.x_inner) + action]);
+  return cat_allowed<MB>(a.mask, vt_row(row, a.inner, a.k_outer, a.k_inner) + action) ? x
+                                                                                     : -INFINITY;
+}
+
 __device__ static inline float cat_nan() { return __uint_as_float(0x7fc00000u); }
 
 // one lane: everything of a row but its alternatives; returns ln S (+inf: no distribution)
-template <typename T, int MB>
-__device__ static inline float cat_finish(const CatArgs& a, int64_t row, int64_t action, CatSum u) {
+__device__ static inline float cat_finish(const CatArgs& a, int64_t row, int64_t action, float x,
+                                          CatSum u) {
   const bool empty = u.s == 0.f;
   const float ls = empty ? INFINITY : logf(u.s);
   if (a.stats != nullptr) {
@@ -176,19 +186,10 @@ __device__ static inline float cat_finish(const CatArgs& a, int64_t row, int64_t
     a.stats[2 * row + 1] = ls;
   }
   if (a.entropy != nullptr) a.entropy[row] = empty ? 0.f : ls - a.inv_t * (u.t / u.s);
-  if (a.log_prob != nullptr) {
-    float lp;
-    if (action >= a.vocab) {
-      lp = cat_nan();
-    } else if (empty || !cat_allowed<T, MB>(a, row, action)) {
-      lp = isnan(ls) ? ls : -INFINITY;
-    } else {
-      const float x = T::one(reinterpret_cast<const typename T::elem*>(
-          a.logits)[vt_row(row, a.inner, a.x_outer, a.x_inner) + action]);
-      lp = (x - u.r) * a.inv_t - ls;
-    }
-    a.log_prob[row] = lp;
-  }
+  if (a.log_prob != nullptr)
+    a.log_prob[row] = action >= a.vocab ? cat_nan()
+                      : empty           ? -INFINITY
+                                        : (x - u.r) * a.inv_t - ls;
   return ls;
 }
 
@@ -296,6 +297,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   const int first = k0 + (TEAM == 64 ? 0 : wave * 64);
   CatTile<T, MB, U> next;
   cat_load<T, MB, U>(x, mk, first + lane, TEAM, k1, skew, a.vocab, next);
+  const float chosen = cat_action_logit<T, MB>(a, row, action);
   if (action < 0) {
     if (a.splits == 1) cat_pad_row(a, row, me);
     return;                        // the whole team returns; the joining launch writes
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   u = cat_wave_join(u, c2);
   if constexpr (TEAM == 64) {
     float ls = 0.f;
-    if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+    if (lane == 0) ls = cat_finish(a, row, action, chosen, u);
     if (TOP) cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
   } else {
     if (lane == 0) { red[0][wave] = u.r; red[1][wave] = u.s; red[2][wave] = u.t; }
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
     }
     if (a.splits == 1) {
       float ls = 0.f;
-      if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+      if (lane == 0) ls = cat_finish(a, row, action, chosen, u);
       if (TOP) cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
     } else {
       if (lane == 0) {
@@ -390,6 +392,7 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
     cat_pad_row(a, row, lane);
     return;
   }
+  const float chosen = cat_action_logit<T, MB>(a, row, action);
   const float c2 = a.inv_t * CAT_LOG2E;
   CatSum u = {CAT_LOWEST, 0.f, 0.f};
   for (int p = lane; p < a.splits; p += 64) {
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
   }
   u = cat_wave_join(u, c2);
   float ls = 0.f;
-  if (lane == 0) ls = cat_finish<T, MB>(a, row, action, u);
+  if (lane == 0) ls = cat_finish(a, row, action, chosen, u);
   if (TOP) {
     CatTop top = {0ull, CAT_EMPTY_KEY, 0, nullptr};
     const int n = a.splits * a.top_k;
@@ -410,6 +413,46 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
     }
     cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
   }
+}
+
+// Few actions: a team of G lanes holds a row in registers, element lane + G i in place i, so the
+// maximum is the row's own and the sums are taken once.
+template <typename T, int MB, int G>
+__global__ void __launch_bounds__(256) aa_categorical_few_kernel(CatArgs a) {
+  constexpr int PER = 256 / G;
+  const int lane = threadIdx.x % G;
+  const int64_t wanted = vt_block() * PER + threadIdx.x / G;
+  // (teams past the last row stay in step with their wave on the last one and store nothing)
+  const int64_t row = wanted < a.rows ? wanted : a.rows - 1;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
+                              vt_row(row, a.inner, a.x_outer, a.x_inner);
+  const int64_t k = MB == 0 ? 0 : vt_row(row, a.inner, a.k_outer, a.k_inner);
+  float v[CAT_FEW];
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; ++i) {
+    const int e = lane + G * i;
+    v[i] = -INFINITY;
+    if (e < a.vocab && cat_allowed<MB>(a.mask, k + e)) v[i] = T::one(x[e]);
+  }
+  const int64_t action = cat_action(a, row);
+  const float chosen = cat_action_logit<T, MB>(a, row, action);
+  const float c2 = a.inv_t * CAT_LOG2E;
+  CatSum u = {CAT_LOWEST, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; ++i) u.r = fmaxf(u.r, v[i]);
+  u.r = wv_group_max<G>(u.r);
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; ++i) {
+    const float d = v[i] - u.r;
+    const float e = cat_exp2(d * c2);
+    u.s += e;
+    u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
+  }
+  u.s = wv_group_sum<G>(u.s);
+  u.t = wv_group_sum<G>(u.t);
+  if (wanted >= a.rows || lane != 0) return;
+  if (action < 0) cat_pad_row(a, row, 0);
+  else cat_finish(a, row, action, chosen, u);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------
@@ -455,11 +498,13 @@ __device__ static inline float cat_grad_one(const CatRow& r, float x) {
   return p * fmaf(r.a1, fmaxf(l, -200.f), r.a0);       // (p is 0 from -150 on)
 }
 
-template <typename T, int MB>
+// TEAM = 64: a wave per row, four rows per workgroup.  TEAM = 256: a workgroup per part of a row.
+template <typename T, int MB, int TEAM>
 __global__ void __launch_bounds__(256) aa_categorical_grad_kernel(CatGradArgs a) {
   constexpr int C = T::C;
-  const int64_t item = vt_block(), row = item / a.blocks;
-  const int block = (int)(item - row * a.blocks);
+  const int64_t item = TEAM == 64 ? vt_block() * 4 + (threadIdx.x >> 6) : vt_block();
+  const int64_t row = TEAM == 64 ? item : item / a.blocks;
+  const int block = TEAM == 64 ? 0 : (int)(item - row * a.blocks);
   if (row >= a.f.rows) return;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.f.logits) +
                               vt_row(row, a.f.inner, a.f.x_outer, a.f.x_inner);
@@ -471,7 +516,8 @@ __global__ void __launch_bounds__(256) aa_categorical_grad_kernel(CatGradArgs a)
   // chunks lie on the destination's 16-byte addresses
   const int skew = (int)(((uintptr_t)dx & 15u) / sizeof(typename T::elem));
   const int chunks = (int)(((int64_t)a.f.vocab + skew + C - 1) / C);
-  for (int k = block * 256 + threadIdx.x; k < chunks; k += a.blocks * 256) {
+  const int step = TEAM == 64 ? 64 : a.blocks * 256;
+  for (int k = block * 256 + threadIdx.x % TEAM; k < chunks; k += step) {
     const int e0 = k * C - skew;
     if (e0 >= 0 && e0 + C <= a.f.vocab) {
       float v[C];
@@ -515,6 +561,35 @@ __global__ void __launch_bounds__(256) aa_categorical_grad_kernel(CatGradArgs a)
   }
 }
 
+// few actions: as the forward call, G lanes a row
+template <typename T, int MB, int G>
+__global__ void __launch_bounds__(256) aa_categorical_few_grad_kernel(CatGradArgs a) {
+  const int lane = threadIdx.x % G;
+  const int64_t row = vt_block() * (256 / G) + threadIdx.x / G;
+  if (row >= a.f.rows) return;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.f.logits) +
+                              vt_row(row, a.f.inner, a.f.x_outer, a.f.x_inner);
+  typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.dx) +
+                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner);
+  const int64_t k = MB == 0 ? 0 : vt_row(row, a.f.inner, a.f.k_outer, a.f.k_inner);
+  float v[CAT_FEW];
+  bool in[CAT_FEW];
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; ++i) {
+    const int e = lane + G * i;
+    in[i] = e < a.f.vocab && cat_allowed<MB>(a.f.mask, k + e);
+    v[i] = in[i] ? T::one(x[e]) : 0.f;
+  }
+  const CatRow r = cat_row_grad(a, row);
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; ++i) {
+    const int e = lane + G * i;
+    float d = cat_grad_one(r, v[i]) + (e == r.action ? r.hit : 0.f);
+    if (r.zero || !in[i]) d = 0.f;
+    if (e < a.f.vocab) dx[e] = T::put(d);
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------
 static int cat_check(const aa_categorical_desc* d) {
   if (d == nullptr || d->rows <= 0 || d->inner <= 0 || d->vocab <= 0 || d->logits == nullptr)
@@ -554,6 +629,13 @@ static CatArgs cat_args(const aa_categorical_desc* d) {
 
 template <typename T, int MB>
 static void cat_launch(const CatArgs& a, hipStream_t st) {
+  if (a.top_k == 0 && a.vocab <= 64 * CAT_FEW) {
+    if (a.vocab <= 8 * CAT_FEW)
+      aa_categorical_few_kernel<T, MB, 8><<<vt_grid((a.rows + 31) / 32), dim3(256), 0, st>>>(a);
+    else
+      aa_categorical_few_kernel<T, MB, 64><<<vt_grid((a.rows + 3) / 4), dim3(256), 0, st>>>(a);
+    return;
+  }
   if (a.vocab <= CAT_WAVE_VOCAB) {
     const dim3 grid = vt_grid((a.rows + 3) / 4);
     if (a.top_k > 0) aa_categorical_kernel<T, MB, 64, true><<<grid, dim3(256), 0, st>>>(a);
@@ -570,12 +652,25 @@ static void cat_launch(const CatArgs& a, hipStream_t st) {
   }
 }
 
+template <typename T, int MB>
+static void cat_launch_grad(const CatGradArgs& g, hipStream_t st) {
+  const int64_t rows = g.f.rows;
+  const dim3 block(256);
+  if (g.f.vocab <= 8 * CAT_FEW)
+    aa_categorical_few_grad_kernel<T, MB, 8><<<vt_grid((rows + 31) / 32), block, 0, st>>>(g);
+  else if (g.f.vocab <= 64 * CAT_FEW)
+    aa_categorical_few_grad_kernel<T, MB, 64><<<vt_grid((rows + 3) / 4), block, 0, st>>>(g);
+  else if (g.f.vocab <= CAT_WAVE_VOCAB)
+    aa_categorical_grad_kernel<T, MB, 64><<<vt_grid((rows + 3) / 4), block, 0, st>>>(g);
+  else
+    aa_categorical_grad_kernel<T, MB, 256><<<vt_grid(rows * g.blocks), block, 0, st>>>(g);
+}
+
 template <typename T>
-static void cat_launch_grad(const CatGradArgs& g, int mask_bytes, hipStream_t st) {
-  const dim3 grid = vt_grid(g.f.rows * g.blocks);
-  if (mask_bytes == 0) aa_categorical_grad_kernel<T, 0><<<grid, dim3(256), 0, st>>>(g);
-  else if (mask_bytes == 1) aa_categorical_grad_kernel<T, 1><<<grid, dim3(256), 0, st>>>(g);
-  else aa_categorical_grad_kernel<T, 4><<<grid, dim3(256), 0, st>>>(g);
+static void cat_launch_grad_mask(const CatGradArgs& g, int mask_bytes, hipStream_t st) {
+  if (mask_bytes == 0) cat_launch_grad<T, 0>(g, st);
+  else if (mask_bytes == 1) cat_launch_grad<T, 1>(g, st);
+  else cat_launch_grad<T, 4>(g, st);
 }
 
 template <typename T>
@@ -636,9 +731,9 @@ int aa_categorical_log_prob_backward(const aa_categorical_desc* d, const float* 
   if (g.f.rows * g.blocks > VT_MAX_BLOCKS) return AA_ERR_RANGE;
   const int mb = d->mask == nullptr ? 0 : d->mask_bytes;
   hipStream_t st = (hipStream_t)stream;
-  if (d->dtype == AA_DT_F32) cat_launch_grad<VtF32>(g, mb, st);
-  else if (d->dtype == AA_DT_BF16) cat_launch_grad<VtBf16>(g, mb, st);
-  else cat_launch_grad<VtF16>(g, mb, st);
+  if (d->dtype == AA_DT_F32) cat_launch_grad_mask<VtF32>(g, mb, st);
+  else if (d->dtype == AA_DT_BF16) cat_launch_grad_mask<VtBf16>(g, mb, st);
+  else cat_launch_grad_mask<VtF16>(g, mb, st);
   return aa_launch_status();
 }
 

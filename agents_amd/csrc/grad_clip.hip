@@ -25,7 +25,7 @@
 // 148 -> 122, 333 MB 200 -> 167; with an update of the clipped tensors behind it 344 -> 348.  Below it
 // costs whoever reads them next: 134 MB 64 -> 64 alone, 137 -> 171 with the update.
 #define CLIP_PAST_CACHE (256ll << 20)
-#define CLIP_FEW 16
+#define CLIP_FEW 32
 
 template <int N>
 struct ClipList {

@@ -57,28 +57,27 @@ __device__ static inline float wv_step(float v, F op) {
   }
 }
 
-// sum over groups of W neighbouring lanes, in each of them the same bits
-template <int W>
-__device__ static inline float wv_group_sum(float v) {
-  const auto add = [](float a, float b) { return a + b; };
-  if constexpr (W >= 2) v = wv_step<1>(v, add);
-  if constexpr (W >= 4) v = wv_step<2>(v, add);
-  if constexpr (W >= 8) v = wv_step<4>(v, add);
-  if constexpr (W >= 16) v = wv_step<8>(v, add);
-  if constexpr (W >= 32) v = wv_step<16>(v, add);
-  if constexpr (W >= 64) v = wv_step<32>(v, add);
+// over groups of W neighbouring lanes, in each of them the same bits
+template <int W, typename F>
+__device__ static inline float wv_group(float v, F op) {
+  if constexpr (W >= 2) v = wv_step<1>(v, op);
+  if constexpr (W >= 4) v = wv_step<2>(v, op);
+  if constexpr (W >= 8) v = wv_step<4>(v, op);
+  if constexpr (W >= 16) v = wv_step<8>(v, op);
+  if constexpr (W >= 32) v = wv_step<16>(v, op);
+  if constexpr (W >= 64) v = wv_step<32>(v, op);
   return v;
 }
-__device__ static inline float wv_sum(float v) { return wv_group_sum<64>(v); }
-__device__ static inline float wv_max(float v) {
-  const auto larger = [](float a, float b) { return fmaxf(a, b); };
-  v = wv_step<1>(v, larger);
-  v = wv_step<2>(v, larger);
-  v = wv_step<4>(v, larger);
-  v = wv_step<8>(v, larger);
-  v = wv_step<16>(v, larger);
-  return wv_step<32>(v, larger);
+template <int W>
+__device__ static inline float wv_group_sum(float v) {
+  return wv_group<W>(v, [](float a, float b) { return a + b; });
 }
+template <int W>
+__device__ static inline float wv_group_max(float v) {
+  return wv_group<W>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ static inline float wv_sum(float v) { return wv_group_sum<64>(v); }
+__device__ static inline float wv_max(float v) { return wv_group_max<64>(v); }
 
 // ---- descending order of 64 keys, one per lane ---------------------------------------------------
 template <int J, typename K>
