@@ -108,11 +108,24 @@ __device__ static inline u64 cat_lane(u64 v, int from) {       // `from` is wave
 }
 
 struct CatTop {
-  u64 list;          // this lane's place of the wave's best 64
+  u64 list;          // this lane's place of the wave's best 64, descending (0: none yet)
   u64 bar;           // a key must exceed it (wave-uniform)
+  float low;         // its value
   int held;          // keys waiting in `buf` (wave-uniform)
-  u64* buf;          // 128 keys of LDS, this wave's own
+  bool sorted;       // `list` holds keys (wave-uniform)
+  u64* buf;          // LDS of this wave's own: 64 keys and what is offered between two flushes
 };
+
+__device__ static inline CatTop cat_top(u64* buf) {
+  return CatTop{0ull, CAT_EMPTY_KEY, -INFINITY, 0, false, buf};
+}
+
+__device__ static inline void cat_top_raise(CatTop& t, u64 bar) {
+  if (bar > t.bar) {
+    t.bar = bar;
+    t.low = cat_key_value(bar);
+  }
+}
 
 __device__ static inline void cat_wave_fence() {
   // LDS of one wave: executed in order, the compiler must keep it so
@@ -121,31 +134,30 @@ __device__ static inline void cat_wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-__device__ static inline void cat_top_merge(CatTop& t, u64 cand, int lane, int k) {
-  t.list = wv_merge_desc(t.list, wv_sort_desc(cand, lane, true), lane);
-  const u64 kth = cat_lane(t.list, k - 1);
-  if (kth > t.bar) t.bar = kth;
-}
-
+// the newest up to 64 waiting keys join the list
 __device__ static inline void cat_top_flush(CatTop& t, int lane, int k) {
-  // the newest up to 64 waiting keys
   const int n = t.held < 64 ? t.held : 64;
   cat_wave_fence();
   const u64 cand = lane < n ? t.buf[t.held - n + lane] : 0ull;
   t.held -= n;
   cat_wave_fence();
-  cat_top_merge(t, cand, lane, k);
+  const u64 order = wv_sort_desc(cand, lane, t.sorted);      // ascending for the merge
+  t.list = t.sorted ? wv_merge_desc(t.list, order, lane) : order;
+  t.sorted = true;
+  cat_top_raise(t, cat_lane(t.list, k - 1));
 }
 
-__device__ static inline void cat_top_offer(CatTop& t, float v, int index, bool real, int lane,
-                                            int k) {
-  const u64 key = cat_key(v, index);
-  const bool in = real && key > t.bar;
+__device__ static inline void cat_top_offer_key(CatTop& t, u64 key, int lane) {
+  const bool in = key > t.bar;
   const u64 b = __ballot(in);
   if (b == 0ull) return;
   if (in) t.buf[t.held + __popcll(b & ((1ull << lane) - 1ull))] = key;
   t.held += __popcll(b);
-  if (t.held >= 64) cat_top_flush(t, lane, k);
+}
+
+// (a comparison of values first: most places hold no candidate; a NaN is none)
+__device__ static inline void cat_top_offer(CatTop& t, float v, int index, int lane) {
+  if (__any(v >= t.low)) cat_top_offer_key(t, v >= t.low ? cat_key(v, index) : 0ull, lane);
 }
 
 // ---- the row's end: log_prob, entropy, stats, alternatives -----------------------------------------
@@ -276,7 +288,7 @@ template <typename T, int MB, int TEAM, bool TOP>
 __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   constexpr int C = T::C, U = MB == 4 ? 2 : 4;
   __shared__ float red[3][4];
-  __shared__ u64 keys[TOP ? 4 : 1][TOP ? 128 : 1];
+  __shared__ u64 keys[TOP ? 4 : 1][TOP ? 64 * (C + 1) : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int me = TEAM == 64 ? lane : threadIdx.x;
   const int64_t item = TEAM == 64 ? vt_block() * 4 + wave : vt_block();
@@ -305,7 +317,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   const float c2 = a.inv_t * CAT_LOG2E;
   const float margin = CAT_MARGIN / c2;
   CatSum u = {CAT_LOWEST, 0.f, 0.f};
-  CatTop top = {0ull, CAT_EMPTY_KEY, 0, TOP ? keys[wave] : nullptr};
+  CatTop top = cat_top(TOP ? keys[wave] : nullptr);
   for (int kb = first; kb < k1; kb += TEAM * U) {          // (wave-uniform)
     const CatTile<T, MB, U> tile = next;
     if (kb + TEAM * U < k1)
@@ -334,16 +346,17 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
       if (kb == first) {
         // k lanes hold a value at or above the k-th of the lanes' maxima, so the row's k best are too
         const unsigned sorted = wv_sort_desc((unsigned)(cat_key(highest, 0) >> 32), lane);
-        const u64 bar = (u64)(unsigned)__builtin_amdgcn_readlane((int)sorted, a.top_k - 1) << 32;
-        if (bar > top.bar) top.bar = bar;
+        cat_top_raise(top, (u64)(unsigned)__builtin_amdgcn_readlane((int)sorted, a.top_k - 1) << 32);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (__any(cat_key(high[i], 0) > top.bar)) {
+        if (__any(high[i] >= top.low)) {
           const int ku = kb + i * TEAM + lane;
 #pragma unroll
           for (int j = 0; j < C; ++j)
-            cat_top_offer(top, v[i][j], ku * C - skew + j, v[i][j] > -INFINITY, lane, a.top_k);
+            cat_top_offer(top, v[i][j], ku * C - skew + j, lane);
+          // (once a chunk: a copy of the sort at every place would not fit the instruction cache)
+          while (top.held >= 64) cat_top_flush(top, lane, a.top_k);
         }
     }
   }
@@ -384,6 +397,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
 // joins the parts of a row: a wave per row
 template <typename T, int MB, bool TOP>
 __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
+  __shared__ u64 keys[TOP ? 128 : 1];
   const int lane = threadIdx.x;
   const int64_t row = vt_block();
   if (row >= a.rows) return;
@@ -404,13 +418,14 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
   float ls = 0.f;
   if (lane == 0) ls = cat_finish(a, row, action, chosen, u);
   if (TOP) {
-    CatTop top = {0ull, CAT_EMPTY_KEY, 0, nullptr};
+    CatTop top = cat_top(keys);
     const int n = a.splits * a.top_k;
     const u64* src = a.part_keys + row * n;
     for (int i = 0; i < n; i += 64) {
-      const u64 key = i + lane < n ? src[i + lane] : 0ull;
-      if (__any(key > top.bar)) cat_top_merge(top, key, lane, a.top_k);
+      cat_top_offer_key(top, i + lane < n ? src[i + lane] : 0ull, lane);
+      if (top.held >= 64) cat_top_flush(top, lane, a.top_k);
     }
+    while (top.held > 0) cat_top_flush(top, lane, a.top_k);
     cat_write_top(a, row, lane, top.list, u.r, __shfl(ls, 0, 64));
   }
 }
