@@ -139,6 +139,28 @@ class Dense(Layer):
         self.name = name
 
 
+class LayerNormalization(Layer):
+    """keras LayerNormalization over the last axis (csrc/layer_norm.hip): gamma (ones), beta (zeros),
+    biased variance; its output is linear."""
+    has_params = True
+    activation = None
+    l2 = 0.0
+
+    def __init__(self, axis=-1, epsilon=1e-3, center=True, scale=True, beta_initializer=None,
+                 gamma_initializer=None, name=None):
+        if axis != -1:
+            raise NotImplementedError("LayerNormalization is over the last axis (axis=-1)")
+        if not (center and scale):
+            raise NotImplementedError("LayerNormalization(center=False / scale=False) is not supported")
+        if not float(epsilon) >= 0:
+            raise ValueError(f"epsilon must not be negative, got {epsilon}")
+        self.epsilon = float(epsilon)
+        # gamma takes the kernel's place among the variables, beta the bias's
+        self.kernel_initializer = get_initializer(gamma_initializer, Constant(1.0))
+        self.bias_initializer = get_initializer(beta_initializer, Zeros())
+        self.name = name
+
+
 class Conv2D(Layer):
     has_params = True
 

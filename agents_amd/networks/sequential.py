@@ -1,4 +1,5 @@
-"""Sequential: a feed-forward stack (Rescale / Conv2D / Flatten / Dense) executed by HIP kernels.
+"""Sequential: a feed-forward stack (Rescale / Conv2D / Flatten / Dense / LayerNormalization) executed
+by HIP kernels.
 
 API follows tf_agents/networks/sequential.py:294 (a Network built from a list of layers, used by
 agents/dqn/examples/v2/train_eval.py:168,364 and examples/dqn/mnih15/dqn_train_eval_atari.py:100).
@@ -123,6 +124,7 @@ class _Slot:
         self.dx_prep = None     # {param index of a conv: input-gradient filter scratch}
         self.dzs = None         # wide-MLP path: d loss / d pre-activation of each layer
         self.wide_in = None     # wide-MLP path: (x, x2) the last forward read its input from
+        self.norm_stats = {}    # {param index of a LayerNormalization: mean and 1 / std of its rows}
 
 
 class Sequential(network.Network):
@@ -178,6 +180,8 @@ class Sequential(network.Network):
                 k = int(np.prod(shape))
                 info.append(((k, l.units), (l.units,), (k,), (l.units,)))
                 shape = (l.units,)
+            elif isinstance(l, L.LayerNormalization):
+                info.append(((shape[-1],), (shape[-1],), shape, shape))
         return info, shape
 
     def create_variables(self, input_tensor_spec=None, device=None, **kwargs):
@@ -254,12 +258,12 @@ class Sequential(network.Network):
     def kernels(self):
         """Kernel (weight-matrix) views, for L2 regularisation over the weights only."""
         self._require_built()
-        return list(self._kviews)
+        return [k for k in self._kviews if k.dim() > 1]
 
     @property
     def kernel_grads(self):
         self._require_built()
-        return list(self._gkviews)
+        return [g for g in self._gkviews if g.dim() > 1]
 
     @property
     def variables(self):
@@ -354,6 +358,9 @@ class Sequential(network.Network):
             s = _Slot()
             for ks, bs, in_shape, out_shape in self._info:
                 s.ys.append(torch.empty((B,) + tuple(out_shape), dtype=torch.float32, device=dev))
+                if len(ks) == 1:
+                    s.norm_stats[len(s.ys) - 1] = torch.empty(
+                        (B,) + tuple(out_shape[:-1]) + (2,), dtype=torch.float32, device=dev)
             s.xs = [None] * len(self._info)
             s.dxs = [None] * len(self._info)
             self._slots[key] = s
@@ -474,6 +481,17 @@ class Sequential(network.Network):
                 else:
                     ops.dense_forward(cur2, self._kviews[pi], self._bviews[pi], l.activation,
                                       s.ys[pi])
+                cur = s.ys[pi]
+                pi += 1
+            elif isinstance(l, L.LayerNormalization):
+                if cur.dtype != torch.float32 or div is not None:
+                    raise NotImplementedError(
+                        "LayerNormalization needs float32 inputs (uint8 / Rescale inputs are fused "
+                        "into a leading Conv2D only)")
+                cur = cur.reshape(s.ys[pi].shape)
+                s.xs[pi] = cur
+                ops.layer_norm_forward(cur, self._kviews[pi], self._bviews[pi], l.epsilon,
+                                       out=s.ys[pi], stats=s.norm_stats[pi])
                 cur = s.ys[pi]
                 pi += 1
         if prep_pending:   # a planned pair was not reached (cannot happen; keeps captures joined)
@@ -1004,6 +1022,19 @@ class Sequential(network.Network):
                                 fork=not (DX_FIRST and i > 0))
                 if dz_next is not None:
                     dz = dz_next
+            elif isinstance(l, L.LayerNormalization):
+                # one pass writes dX (with the layer below's activation gradient) and the sums of
+                # the weights' gradients, both on the caller's stream
+                dx = s.dxs[i] if i > 0 else input_grad
+                if dx is not None or param_grads:
+                    ops.layer_norm_backward(
+                        dz.view(x.shape), x, self._kviews[i], s.norm_stats[i],
+                        dx=None if dx is None else dx.view(x.shape), dgamma=self._gkviews[i],
+                        dbeta=self._gbviews[i], mask_act=prev_act, param_grads=param_grads,
+                        input_grad=dx is not None)
+                issue_late_prep()
+                if i > 0:
+                    dz = s.dxs[i]
             else:
                 F = ks[3]
                 dz2 = dz.view(-1, F)

@@ -11,7 +11,7 @@ mask (masked logits -> dtype.min), a Philox uniform per env, and the epsilon mix
 import numpy as np
 import torch
 
-from agents_amd import _lib
+from agents_amd import _lib, ops
 from agents_amd.policies import tf_policy
 from agents_amd.trajectories import policy_step
 from agents_amd.utils import graph, nest_utils
@@ -25,8 +25,9 @@ def _action_bounds(action_spec):
 
 
 class Categorical:
-    """What `policy.distribution(time_step).action` exposes of tfp Categorical: `logits` [B, A]
-    and `mode()` (first arg-max, greedy_policy.py:70-89)."""
+    """What `policy.distribution(time_step).action` exposes of tfp Categorical: `logits` [B, A],
+    `mode()` (first arg-max, greedy_policy.py:70-89), `log_prob(actions)` and `entropy()` [B], and the
+    most likely actions (`most_likely`)."""
 
     def __init__(self, logits, policy):
         self.logits = logits
@@ -34,6 +35,22 @@ class Categorical:
 
     def mode(self):
         return self._policy.select(self.logits, None, 0.0)
+
+    def log_prob(self, actions):
+        """Log-probabilities of actions of the policy's action spec: [B] int32 / int64, or [B, 1] for
+        a spec of shape (1,)."""
+        r = ops.categorical_log_prob(self.logits, actions.reshape(self.logits.shape[0]),
+                                     first_action=self._policy._lo)
+        return r.log_prob
+
+    def entropy(self):
+        return ops.categorical_log_prob(self.logits).entropy
+
+    def most_likely(self, k):
+        """(actions [B, k] int64, log-probabilities [B, k]) by descending probability, equal ones by
+        ascending action; k is cut to the number of actions."""
+        r = ops.categorical_log_prob(self.logits, top_k=k)
+        return r.top_ids + self._policy._lo, r.top_log_prob
 
 
 def distribution_of(policy, time_step, temperature):

@@ -6,6 +6,8 @@
   Periodically                 common.py:450-507
   element_wise_huber_loss / element_wise_squared_loss   common.py:1199-1208
   Checkpointer                 common.py:1045-1100 (format is ours: torch.save of state dicts)
+  log_probability / entropy    sums over a nest of action distributions (Categorical.log_prob /
+                               entropy: csrc/categorical.hip)
 """
 import functools
 import os
@@ -15,6 +17,7 @@ import zipfile
 import torch
 
 from agents_amd import _lib
+from agents_amd.utils import nest_utils
 
 
 def function(*args, **kwargs):
@@ -135,6 +138,20 @@ def soft_variables_update(source_variables, target_variables, tau=1.0, tau_non_t
             _lib.require_cuda(s, t)
             _lib.check(lib.aa_soft_update(t.data_ptr(), s.data_ptr(), t.numel(), float(tau),
                                           _lib.stream_ptr()), "aa_soft_update")
+
+
+def log_probability(distributions, actions, action_spec=None):
+    """Sum over the nest of the log-probabilities of `actions`, one value per batch row."""
+    nest_utils.assert_same_structure(distributions, actions)
+    parts = [d.log_prob(a) for d, a in zip(nest_utils.flatten(distributions),
+                                           nest_utils.flatten(actions))]
+    return functools.reduce(lambda x, y: x + y, parts)
+
+
+def entropy(distributions, action_spec=None):
+    """Sum over the nest of the distributions' entropies, one value per batch row."""
+    return functools.reduce(lambda x, y: x + y,
+                            [d.entropy() for d in nest_utils.flatten(distributions)])
 
 
 def weak_method(bound):
