@@ -113,6 +113,8 @@ def test_entry_points_refuse(lib):
         setattr(b, k, v)
         assert lib.aa_layer_norm_forward(ctypes.byref(b), None) == -22, k
     ln.dy, ln.stats, ln.dx, ln.dgamma = 64, 64, 64, 64
+    assert lib.aa_layer_norm_backward_workspace_bytes(ctypes.byref(ln)) == 0     # one workgroup
+    ln.rows = 5000
     need = lib.aa_layer_norm_backward_workspace_bytes(ctypes.byref(ln))
     assert need > 0
     assert lib.aa_layer_norm_backward(ctypes.byref(ln), None, 0, None) == -34
