@@ -477,12 +477,24 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     out = out_guard.o = PySequence_List(a[4]);
     if (out == nullptr) throw Raised{};
   } else if (scale) {
+    // pieces of one allocation (as networks keep their gradients), each on a cache line of its own:
+    // an allocation of each took 0.8 us a tensor, most of a call on small gradients
+    const int64_t line = 128 / t0.element_size();
+    int64_t total = 0;
+    for (size_t i = 0; i < n; ++i) total += (sizes[i] + line - 1) / line * line;
+    const at::Tensor flat = at::empty({total}, t0.options());
     out = out_guard.o = PyList_New((Py_ssize_t)n);
     if (out == nullptr) throw Raised{};
+    int64_t at = 0;
     for (size_t i = 0; i < n; ++i) {
-      const at::Tensor o = at::empty(ts[i]->sizes(), t0.options());
+      auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(),
+                                                       flat.dtype());
+      impl->set_storage_offset(at);
+      impl->set_sizes_contiguous(ts[i]->sizes());
+      const at::Tensor o(std::move(impl));
       dst[i] = o.data_ptr();
       PyList_SET_ITEM(out, (Py_ssize_t)i, wrap(o));
+      at += (sizes[i] + line - 1) / line * line;
     }
   } else {
     out = out_guard.o = Py_None;

@@ -894,8 +894,9 @@ def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dent
 def clip_by_global_norm(tensors, clip_norm, out=None):
     """tf.clip_by_global_norm: ([t * clip_norm / max(global norm, clip_norm)], global norm) of a list
     of contiguous float32 / bfloat16 / float16 tensors of one type (csrc/grad_clip.hip).  `out`: a
-    list that receives the clipped tensors, `tensors` itself for clipping in place.  The norm is a
-    float32 scalar on the device; one that is not finite makes every clipped value NaN."""
+    list that receives the clipped tensors, `tensors` itself for clipping in place; without it they
+    are pieces of one new allocation.  The norm is a float32 scalar on the device; one that is not
+    finite makes every clipped value NaN."""
     return (_token_ops or _bind()).clip(tensors, clip_norm, False, True, out, "clip_by_global_norm")
 
 
