@@ -24,6 +24,7 @@
 #define CAT_LN2 0.6931471805599453f
 #define CAT_FEW 8                  // elements a lane holds of a row of few actions (up to 64 x 8)
 #define CAT_WAVE_VOCAB 4096        // up to here a wave takes a row, beyond a workgroup
+#define CAT_SPLIT_ROWS 256         // (one workgroup a CU)
 #define CAT_SPLIT_BLOCKS 1024      // workgroups that fill the machine
 // A gradient of this many bytes is stored past the caches: with the logits it exceeds the 256 MB of the
 // memory-side cache, and its dirty lines would be written back under the next reads.  Forward and
@@ -240,47 +241,48 @@ struct CatTile {
   unsigned m[U][W];
 };
 
-template <typename T, int MB, int U>
-__device__ static inline void cat_load(const typename T::elem* x, const uint8_t* mk, int k, int team,
-                                       int k1, int skew, int vocab, CatTile<T, MB, U>& t) {
+// `k`: this lane's first chunk, `kb`: its wave's; chunks from k1 on read as -inf
+template <typename T, int MB, int U, int TEAM>
+__device__ static inline void cat_load(const typename T::elem* x, const uint8_t* mk, int kb, int lane,
+                                       int k1, int skew, CatTile<T, MB, U>& t) {
   constexpr int C = T::C;
+  const int e0 = (kb + lane) * C - skew;
+  if (kb + (U - 1) * TEAM + 64 <= k1) {                    // (wave-uniform: all there)
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int ku = k + u * team, e0 = ku * C - skew;
-    t.q[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (ku < k1 && e0 >= 0 && e0 + C <= vocab) {
-      t.q[u] = vt_load16(x + e0);
-      if (MB != 0) __builtin_memcpy(t.m[u], mk + (int64_t)MB * e0, MB * C);
+    for (int u = 0; u < U; ++u) {
+      t.q[u] = vt_load16(x + e0 + u * TEAM * C);
+      if (MB != 0) __builtin_memcpy(t.m[u], mk + (int64_t)MB * (e0 + u * TEAM * C), MB * C);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned w = T::LOWEST_WORD;
+      t.q[u] = make_uint4(w, w, w, w);
+      if (kb + lane + u * TEAM < k1) {
+        t.q[u] = vt_load16(x + e0 + u * TEAM * C);
+        if (MB != 0) __builtin_memcpy(t.m[u], mk + (int64_t)MB * (e0 + u * TEAM * C), MB * C);
+      }
     }
   }
 }
 
-// chunk u as fp32, -inf where it is masked or not there
+// chunk u as fp32, -inf where it is masked
 template <typename T, int MB, int U>
-__device__ static inline void cat_values(const typename T::elem* x, const uint8_t* mk, int ku, int k1,
-                                         int skew, int vocab, const CatTile<T, MB, U>& t, int u,
-                                         float (&v)[T::C]) {
-  constexpr int C = T::C;
-  const int e0 = ku * C - skew;
-  if (ku < k1 && e0 >= 0 && e0 + C <= vocab) {
-    T::widen(t.q[u], v);
+__device__ static inline void cat_values(const CatTile<T, MB, U>& t, int u, float (&v)[T::C]) {
+  T::widen(t.q[u], v);
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      if (MB == 1 && ((t.m[u][j / 4] >> (8 * (j % 4))) & 0xffu) == 0u) v[j] = -INFINITY;
-      if (MB == 4 && t.m[u][j] == 0u) v[j] = -INFINITY;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int e = e0 + j;
-      v[j] = -INFINITY;
-      if (ku < k1 && e >= 0 && e < vocab) {
-        v[j] = T::one(x[e]);
-        if (MB == 1 && mk[e] == 0) v[j] = -INFINITY;
-        if (MB == 4 && reinterpret_cast<const int32_t*>(mk)[e] == 0) v[j] = -INFINITY;
-      }
-    }
+  for (int j = 0; j < T::C; ++j) {
+    if (MB == 1 && ((t.m[u][j / 4] >> (8 * (j % 4))) & 0xffu) == 0u) v[j] = -INFINITY;
+    if (MB == 4 && t.m[u][j] == 0u) v[j] = -INFINITY;
   }
+}
+
+// a value into the sums of its lane
+__device__ static inline void cat_add(CatSum& u, float v, float c2) {
+  const float d = v - u.r;
+  const float e = cat_exp2(d * c2);
+  u.s += e;
+  u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
 }
 
 // TEAM = 64: a wave per row, four rows per workgroup.  TEAM = 256: a workgroup per part of a row.
@@ -300,15 +302,19 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
                               vt_row(row, a.inner, a.x_outer, a.x_inner);
   const uint8_t* mk = MB == 0 ? nullptr : reinterpret_cast<const uint8_t*>(a.mask) +
                                               MB * vt_row(row, a.inner, a.k_outer, a.k_inner);
-  // chunks lie on 16-byte addresses: chunk k holds elements k C - skew ..
+  // Whole chunks lie on 16-byte addresses: chunk k holds elements k C - skew ..; the elements in front
+  // of the first and behind the last one are taken one by one, by the first wave of their part.
   const int skew = (int)(((uintptr_t)x & 15u) / sizeof(typename T::elem));
-  const int chunks = (int)(((int64_t)a.vocab + skew + C - 1) / C);
+  const int whole0 = skew > 0 ? 1 : 0;
+  int whole1 = (int)(((int64_t)a.vocab + skew) / C);
+  if (whole1 < whole0) whole1 = whole0;
+  const int chunks = whole1 - whole0;
   const int each = TEAM == 64 ? chunks : (chunks + a.splits - 1) / a.splits;
-  const int k0 = part * each;
-  const int k1 = k0 + each < chunks ? k0 + each : chunks;
+  const int k0 = whole0 + part * each;
+  const int k1 = k0 + each < whole1 ? k0 + each : whole1;
   const int first = k0 + (TEAM == 64 ? 0 : wave * 64);
   CatTile<T, MB, U> next;
-  cat_load<T, MB, U>(x, mk, first + lane, TEAM, k1, skew, a.vocab, next);
+  if (first < k1) cat_load<T, MB, U, TEAM>(x, mk, first, lane, k1, skew, next);
   const float chosen = cat_action_logit<T, MB>(a, row, action);
   if (action < 0) {
     if (a.splits == 1) cat_pad_row(a, row, me);
@@ -318,15 +324,26 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
   const float margin = CAT_MARGIN / c2;
   CatSum u = {CAT_LOWEST, 0.f, 0.f};
   CatTop top = cat_top(TOP ? keys[wave] : nullptr);
+  if ((TEAM == 64 || wave == 0) && (part == 0 || part == a.splits - 1)) {
+    const int head = part == 0 ? whole0 * C - skew : 0;                  // (skew 0: none)
+    const int tail = part == a.splits - 1 ? whole1 * C - skew : a.vocab;
+    // lanes 0 .. 31 the front, 32 .. 63 the end: fewer than 8 elements each
+    const int e = lane < 32 ? lane : tail + lane - 32;
+    const bool here = lane < 32 ? e < head && e < a.vocab : e >= head && e < a.vocab;
+    float v = -INFINITY;
+    if (here && cat_allowed<MB>(mk, e)) v = T::one(x[e]);
+    if (v > u.r + margin) u.r = v;
+    cat_add(u, v, c2);
+    if (TOP) cat_top_offer(top, v, e, lane);
+  }
   for (int kb = first; kb < k1; kb += TEAM * U) {          // (wave-uniform)
     const CatTile<T, MB, U> tile = next;
-    if (kb + TEAM * U < k1)
-      cat_load<T, MB, U>(x, mk, kb + TEAM * U + lane, TEAM, k1, skew, a.vocab, next);
+    if (kb + TEAM * U < k1) cat_load<T, MB, U, TEAM>(x, mk, kb + TEAM * U, lane, k1, skew, next);
     float v[U][C], high[U];
     float highest = -INFINITY;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      cat_values<T, MB, U>(x, mk, kb + i * TEAM + lane, k1, skew, a.vocab, tile, i, v[i]);
+      cat_values<T, MB, U>(tile, i, v[i]);
       high[i] = v[i][0];
 #pragma unroll
       for (int j = 1; j < C; ++j) high[i] = fmaxf(high[i], v[i][j]);
@@ -336,12 +353,7 @@ __global__ void __launch_bounds__(256) aa_categorical_kernel(CatArgs a) {
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const float d = v[i][j] - u.r;
-        const float e = cat_exp2(d * c2);
-        u.s += e;
-        u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
-      }
+      for (int j = 0; j < C; ++j) cat_add(u, v[i][j], c2);
     if (TOP) {
       if (kb == first) {
         // k lanes hold a value at or above the k-th of the lanes' maxima, so the row's k best are too
@@ -430,8 +442,49 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
   }
 }
 
-// Few actions: a team of G lanes holds a row in registers, element lane + G i in place i, so the
-// maximum is the row's own and the sums are taken once.
+// Few actions: a team of G lanes holds a row in registers, CAT_FEW neighbouring elements a lane, so the
+// maximum is the row's own and the sums are taken once.  Rows lie behind each other, so 16-byte loads of
+// neighbouring teams share cache lines (elements G apart took 59 us a pass for 148248 f32 rows of 58).
+
+// elements e0 .. of a row and which of them exist and are allowed, one bit each
+template <typename T, int MB>
+__device__ static inline unsigned cat_few_load(const CatArgs& a, int64_t row, int e0,
+                                               float (&v)[CAT_FEW]) {
+  constexpr int C = T::C;
+  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
+                              vt_row(row, a.inner, a.x_outer, a.x_inner) + e0;
+  const int n = a.vocab - e0;
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; i += C) {
+    float w[C];
+    if (i + C <= n) T::widen(vt_load16(x + i), w);
+    else vt_load_part<T>(x + i, n - i, 0.f, w);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[i + j] = w[j];
+  }
+  unsigned in = n >= CAT_FEW ? (1u << CAT_FEW) - 1u : n > 0 ? (1u << n) - 1u : 0u;
+  if constexpr (MB != 0) {
+    const uint8_t* mk = reinterpret_cast<const uint8_t*>(a.mask) +
+                        MB * (vt_row(row, a.inner, a.k_outer, a.k_inner) + e0);
+    unsigned m[MB * CAT_FEW / 4];
+    if (n >= CAT_FEW) {
+      __builtin_memcpy(m, mk, MB * CAT_FEW);
+    } else {
+#pragma unroll
+      for (int j = 0; j < MB * CAT_FEW / 4; ++j) m[j] = 0u;
+#pragma unroll
+      for (int j = 0; j < CAT_FEW; ++j)
+        if (j < n && cat_allowed<MB>(mk, j)) m[MB * j / 4] |= MB == 1 ? 1u << (8 * (j % 4)) : 1u;
+    }
+#pragma unroll
+    for (int j = 0; j < CAT_FEW; ++j) {
+      const unsigned w = MB == 1 ? (m[j / 4] >> (8 * (j % 4))) & 0xffu : m[MB * j / 4];
+      if (w == 0u) in &= ~(1u << j);
+    }
+  }
+  return in;
+}
+
 template <typename T, int MB, int G>
 __global__ void __launch_bounds__(256) aa_categorical_few_kernel(CatArgs a) {
   constexpr int PER = 256 / G;
@@ -439,16 +492,11 @@ __global__ void __launch_bounds__(256) aa_categorical_few_kernel(CatArgs a) {
   const int64_t wanted = vt_block() * PER + threadIdx.x / G;
   // (teams past the last row stay in step with their wave on the last one and store nothing)
   const int64_t row = wanted < a.rows ? wanted : a.rows - 1;
-  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
-                              vt_row(row, a.inner, a.x_outer, a.x_inner);
-  const int64_t k = MB == 0 ? 0 : vt_row(row, a.inner, a.k_outer, a.k_inner);
   float v[CAT_FEW];
+  const unsigned in = cat_few_load<T, MB>(a, row, lane * CAT_FEW, v);
 #pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i) {
-    const int e = lane + G * i;
-    v[i] = -INFINITY;
-    if (e < a.vocab && cat_allowed<MB>(a.mask, k + e)) v[i] = T::one(x[e]);
-  }
+  for (int i = 0; i < CAT_FEW; ++i)
+    if (((in >> i) & 1u) == 0u) v[i] = -INFINITY;
   const int64_t action = cat_action(a, row);
   const float chosen = cat_action_logit<T, MB>(a, row, action);
   const float c2 = a.inv_t * CAT_LOG2E;
@@ -582,26 +630,24 @@ __global__ void __launch_bounds__(256) aa_categorical_few_grad_kernel(CatGradArg
   const int lane = threadIdx.x % G;
   const int64_t row = vt_block() * (256 / G) + threadIdx.x / G;
   if (row >= a.f.rows) return;
-  const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.f.logits) +
-                              vt_row(row, a.f.inner, a.f.x_outer, a.f.x_inner);
-  typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.dx) +
-                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner);
-  const int64_t k = MB == 0 ? 0 : vt_row(row, a.f.inner, a.f.k_outer, a.f.k_inner);
+  const int e0 = lane * CAT_FEW, n = a.f.vocab - e0;
   float v[CAT_FEW];
-  bool in[CAT_FEW];
-#pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i) {
-    const int e = lane + G * i;
-    in[i] = e < a.f.vocab && cat_allowed<MB>(a.f.mask, k + e);
-    v[i] = in[i] ? T::one(x[e]) : 0.f;
-  }
+  const unsigned in = cat_few_load<T, MB>(a.f, row, e0, v);
   const CatRow r = cat_row_grad(a, row);
 #pragma unroll
   for (int i = 0; i < CAT_FEW; ++i) {
-    const int e = lane + G * i;
-    float d = cat_grad_one(r, v[i]) + (e == r.action ? r.hit : 0.f);
-    if (r.zero || !in[i]) d = 0.f;
-    if (e < a.f.vocab) dx[e] = T::put(d);
+    v[i] = cat_grad_one(r, v[i]) + (e0 + i == r.action ? r.hit : 0.f);
+    if (r.zero || ((in >> i) & 1u) == 0u) v[i] = 0.f;
+  }
+  typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.dx) +
+                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner) + e0;
+#pragma unroll
+  for (int i = 0; i < CAT_FEW; i += T::C) {
+    float w[T::C];
+#pragma unroll
+    for (int j = 0; j < T::C; ++j) w[j] = v[i + j];
+    if (i + T::C <= n) vt_store16(dx + i, T::pack(w));
+    else vt_store_part<T>(dx + i, n - i, w);
   }
 }
 
@@ -619,9 +665,13 @@ static int cat_check(const aa_categorical_desc* d) {
   return AA_OK;
 }
 
+// Rows are split where a workgroup for each leaves CUs idle (up to CAT_SPLIT_ROWS rows) and a row is
+// longer than what a workgroup reads while the joining launch runs (32 KB).  us without / with:
+// bf16 16000 x 64 rows 5.6 / 6.9, 50001 x 64 11.4 / 7.5, x 256 13.1 / 14.3, x 384 16.3 / 18.8,
+// 131072 x 1 19 / 6.3, x 256 20.8 / 19.3, x 384 29 / 32; f32 131072 x 192 42 / 29, x 384 54 / 50.
 static int cat_splits(const aa_categorical_desc* d) {
-  if (d->vocab <= CAT_WAVE_VOCAB) return 1;
   const int per = d->dtype == AA_DT_F32 ? 4 : 8;
+  if (d->rows > CAT_SPLIT_ROWS || d->vocab <= 2048 * per) return 1;
   int64_t want = (CAT_SPLIT_BLOCKS + d->rows - 1) / d->rows;
   const int64_t most = (d->vocab / per + 1023) / 1024;     // four rounds of a workgroup at least
   if (want > most) want = most;
@@ -642,13 +692,19 @@ static CatArgs cat_args(const aa_categorical_desc* d) {
   return a;
 }
 
+// lanes that hold a row of few actions
+static int cat_few_team(int vocab) {
+  return vocab <= 8 * CAT_FEW ? 8 : vocab <= 16 * CAT_FEW ? 16 : 64;
+}
+
 template <typename T, int MB>
 static void cat_launch(const CatArgs& a, hipStream_t st) {
   if (a.top_k == 0 && a.vocab <= 64 * CAT_FEW) {
-    if (a.vocab <= 8 * CAT_FEW)
-      aa_categorical_few_kernel<T, MB, 8><<<vt_grid((a.rows + 31) / 32), dim3(256), 0, st>>>(a);
-    else
-      aa_categorical_few_kernel<T, MB, 64><<<vt_grid((a.rows + 3) / 4), dim3(256), 0, st>>>(a);
+    const int team = cat_few_team(a.vocab);
+    const dim3 grid = vt_grid((a.rows + 256 / team - 1) / (256 / team));
+    if (team == 8) aa_categorical_few_kernel<T, MB, 8><<<grid, dim3(256), 0, st>>>(a);
+    else if (team == 16) aa_categorical_few_kernel<T, MB, 16><<<grid, dim3(256), 0, st>>>(a);
+    else aa_categorical_few_kernel<T, MB, 64><<<grid, dim3(256), 0, st>>>(a);
     return;
   }
   if (a.vocab <= CAT_WAVE_VOCAB) {
@@ -671,10 +727,14 @@ template <typename T, int MB>
 static void cat_launch_grad(const CatGradArgs& g, hipStream_t st) {
   const int64_t rows = g.f.rows;
   const dim3 block(256);
-  if (g.f.vocab <= 8 * CAT_FEW)
-    aa_categorical_few_grad_kernel<T, MB, 8><<<vt_grid((rows + 31) / 32), block, 0, st>>>(g);
+  const int team = cat_few_team(g.f.vocab);
+  const dim3 few = vt_grid((rows + 256 / team - 1) / (256 / team));
+  if (team == 8)
+    aa_categorical_few_grad_kernel<T, MB, 8><<<few, block, 0, st>>>(g);
+  else if (team == 16)
+    aa_categorical_few_grad_kernel<T, MB, 16><<<few, block, 0, st>>>(g);
   else if (g.f.vocab <= 64 * CAT_FEW)
-    aa_categorical_few_grad_kernel<T, MB, 64><<<vt_grid((rows + 3) / 4), block, 0, st>>>(g);
+    aa_categorical_few_grad_kernel<T, MB, 64><<<few, block, 0, st>>>(g);
   else if (g.f.vocab <= CAT_WAVE_VOCAB)
     aa_categorical_grad_kernel<T, MB, 64><<<vt_grid((rows + 3) / 4), block, 0, st>>>(g);
   else

@@ -493,14 +493,19 @@ __global__ void __launch_bounds__(256) aa_layer_norm_dw_wide_kernel(LnArgs a) {
       }
     }
   }
-  float* out = a.partial + (int64_t)blockIdx.y * 2 * a.width;
+  float* og = a.partial + (int64_t)blockIdx.y * 2 * a.width;
+  float* ob = og + a.width;
+  if (gridDim.y == 1) {            // nothing to join
+    og = a.dgamma;
+    ob = a.dbeta;
+  }
 #pragma unroll
   for (int j = 0; j < C; j += 4) {
     const float g[4] = {dg[j], dg[j + 1], dg[j + 2], dg[j + 3]};
     const float b[4] = {db[j], db[j + 1], db[j + 2], db[j + 3]};
     if (c + j < a.width) {
-      ln_put<VtF32>(out, c + j, a.width, g);
-      ln_put<VtF32>(out + a.width, c + j, a.width, b);
+      if (og != nullptr) ln_put<VtF32>(og, c + j, a.width, g);
+      if (ob != nullptr) ln_put<VtF32>(ob, c + j, a.width, b);
     }
   }
 }
@@ -596,7 +601,7 @@ static int ln_check(const aa_layer_norm_desc* d) {
 
 // whether the weights' gradients pass through partials
 static bool ln_joins(const aa_layer_norm_desc* d) {
-  return ln_bwd_team(d->width) == 0 || ln_groups(d->rows, d->width) > 1;
+  return ln_groups(d->rows, d->width) > 1;
 }
 
 static LnArgs ln_args(const aa_layer_norm_desc* d) {

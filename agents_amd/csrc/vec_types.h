@@ -12,6 +12,7 @@ typedef float vt_f32x2 __attribute__((ext_vector_type(2)));
 struct VtF32 {
   typedef float elem;
   static constexpr int C = 4;
+  static constexpr unsigned LOWEST_WORD = 0xff800000u;       // -inf in every element of a word
   __device__ static inline float one(elem e) { return e; }
   __device__ static inline elem put(float f) { return f; }
   __device__ static inline void widen(const uint4& q, float (&v)[C]) {
@@ -27,6 +28,7 @@ struct VtF32 {
 struct VtBf16 {
   typedef __bf16 elem;
   static constexpr int C = 8;
+  static constexpr unsigned LOWEST_WORD = 0xff80ff80u;
   __device__ static inline float one(elem e) { return (float)e; }
   __device__ static inline elem put(float f) { return (__bf16)f; }   // round to nearest even
   __device__ static inline void widen(const uint4& q, float (&v)[C]) {
@@ -51,6 +53,7 @@ struct VtBf16 {
 struct VtF16 {
   typedef _Float16 elem;
   static constexpr int C = 8;
+  static constexpr unsigned LOWEST_WORD = 0xfc00fc00u;
   __device__ static inline float one(elem e) { return (float)e; }
   __device__ static inline elem put(float f) { return (_Float16)f; }
   __device__ static inline void widen(const uint4& q, float (&v)[C]) {
