@@ -141,7 +141,7 @@ aa_clip_scale_kernel(ClipList<N> L, const double* __restrict__ partial, int64_t 
     }
   }
   // the factor is rounded to fp32 once; no clipping gives exactly 1
-  const float f = nrm <= clip ? 1.f : isfinite(nrm) ? (float)(clip / nrm) : NAN;
+  const float f = !isfinite(nrm) ? NAN : nrm <= clip ? 1.f : (float)(clip / nrm);
   auto put = [&](const uint4& q, int64_t at) {
     float v[C];
     T::widen(q, v);

@@ -595,7 +595,7 @@ static int ln_check(const aa_layer_norm_desc* d) {
     return AA_ERR_INVALID;
   if (d->dtype < AA_DT_F32 || d->dtype > AA_DT_F16) return AA_ERR_INVALID;
   if (d->mask_act < AA_ACT_NONE || d->mask_act > AA_ACT_TANH) return AA_ERR_INVALID;
-  if (d->width > (1 << 30) || d->rows > VT_MAX_BLOCKS) return AA_ERR_RANGE;
+  if (d->width > (1 << 29) || d->rows > VT_MAX_BLOCKS) return AA_ERR_RANGE;
   return AA_OK;
 }
 

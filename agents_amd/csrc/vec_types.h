@@ -111,7 +111,8 @@ __device__ static inline void vt_store_part(typename T::elem* p, int n, const fl
 __device__ static inline int64_t vt_row(int64_t r, int64_t inner, int64_t ld_outer,
                                         int64_t ld_inner) {
   if (inner == 1) return r * ld_outer;
-  const int64_t o = r / inner;
+  // (a quotient of 32 bits where it can be one: a fifth of the instructions)
+  const int64_t o = ((r | inner) >> 32) == 0 ? (int64_t)((uint32_t)r / (uint32_t)inner) : r / inner;
   return o * ld_outer + (r - o * inner) * ld_inner;
 }
 

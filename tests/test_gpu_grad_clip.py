@@ -119,6 +119,10 @@ def test_not_finite(dev, bad):
     got, norms = ops.clip_by_norms(ts, 0.1)
     assert got[1].isnan().all() and not got[0].isnan().any() and not got[2].isnan().any()
     check(ts, 0.1, True, got, norms)
+    # whatever the limit
+    assert ops.clip_by_global_norm(ts, float("inf"))[0][0].isnan().all()
+    ts[1][8999] = 0.0
+    assert torch.equal(ops.clip_by_global_norm(ts, float("inf"))[0][0], ts[0])
 
 
 def test_same_bits_on_two_streams_and_in_a_graph(dev):
