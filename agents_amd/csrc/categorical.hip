@@ -22,7 +22,7 @@
 #define CAT_LOWEST (-3.402823466e+38f)
 #define CAT_LOG2E 1.4426950408889634f
 #define CAT_LN2 0.6931471805599453f
-#define CAT_FEW 8                  // elements a lane holds of a row of few actions (up to 64 x 8)
+#define CAT_FEW 512                // up to here a row is held in registers
 #define CAT_WAVE_VOCAB 4096        // up to here a wave takes a row, beyond a workgroup
 #define CAT_SPLIT_ROWS 256         // (one workgroup a CU)
 #define CAT_SPLIT_BLOCKS 1024      // workgroups that fill the machine
@@ -446,75 +446,68 @@ __global__ void __launch_bounds__(64) aa_categorical_join_kernel(CatArgs a) {
   }
 }
 
-// Few actions: a team of G lanes holds a row in registers, CAT_FEW neighbouring elements a lane, so the
-// maximum is the row's own and the sums are taken once.  Rows lie behind each other, so 16-byte loads of
-// neighbouring teams share cache lines (elements G apart took 59 us a pass for 148248 f32 rows of 58).
+// Few actions: a team of G lanes holds a row in registers, F elements a lane in chunks G apart, so the
+// maximum is the row's own and the sums are taken once.  Bound by the instructions around a row (its
+// reductions, its logarithm), so several rows share a wave: bf16 38000x300 takes 23 us with a wave a row.
 
-// elements e0 .. of a row and which of them exist and are allowed, one bit each
-template <typename T, int MB>
-__device__ static inline unsigned cat_few_load(const CatArgs& a, int64_t row, int e0,
-                                               float (&v)[CAT_FEW]) {
+// the lane's elements and which of them exist and are allowed, one bit each
+template <typename T, int MB, int G, int F>
+__device__ static inline unsigned cat_few_load(const CatArgs& a, int64_t row, int lane, float (&v)[F]) {
   constexpr int C = T::C;
   const typename T::elem* x = reinterpret_cast<const typename T::elem*>(a.logits) +
-                              vt_row(row, a.inner, a.x_outer, a.x_inner) + e0;
-  const int n = a.vocab - e0;
+                              vt_row(row, a.inner, a.x_outer, a.x_inner);
+  const uint8_t* mk = MB == 0 ? nullptr : reinterpret_cast<const uint8_t*>(a.mask) +
+                                              MB * vt_row(row, a.inner, a.k_outer, a.k_inner);
+  unsigned in = 0u;
 #pragma unroll
-  for (int i = 0; i < CAT_FEW; i += C) {
+  for (int i = 0; i < F / C; ++i) {
+    const int e0 = (i * G + lane) * C, n = a.vocab - e0;
     float w[C];
-    if (i + C <= n) T::widen(vt_load16(x + i), w);
-    else vt_load_part<T>(x + i, n - i, 0.f, w);
+    unsigned bits = (1u << C) - 1u;
+    if (n >= C) {
+      T::widen(vt_load16(x + e0), w);
+      if constexpr (MB != 0) {
+        unsigned m[MB * C / 4];
+        __builtin_memcpy(m, mk + MB * e0, MB * C);
 #pragma unroll
-    for (int j = 0; j < C; ++j) v[i + j] = w[j];
-  }
-  unsigned in = n >= CAT_FEW ? (1u << CAT_FEW) - 1u : n > 0 ? (1u << n) - 1u : 0u;
-  if constexpr (MB != 0) {
-    const uint8_t* mk = reinterpret_cast<const uint8_t*>(a.mask) +
-                        MB * (vt_row(row, a.inner, a.k_outer, a.k_inner) + e0);
-    unsigned m[MB * CAT_FEW / 4];
-    if (n >= CAT_FEW) {
-      __builtin_memcpy(m, mk, MB * CAT_FEW);
+        for (int j = 0; j < C; ++j)
+          if (MB == 1 ? ((m[j / 4] >> (8 * (j % 4))) & 0xffu) == 0u : m[MB * j / 4] == 0u)
+            bits &= ~(1u << j);
+      }
     } else {
+      vt_load_part<T>(x + e0, n, 0.f, w);
 #pragma unroll
-      for (int j = 0; j < MB * CAT_FEW / 4; ++j) m[j] = 0u;
-#pragma unroll
-      for (int j = 0; j < CAT_FEW; ++j)
-        if (j < n && cat_allowed<MB>(mk, j)) m[MB * j / 4] |= MB == 1 ? 1u << (8 * (j % 4)) : 1u;
+      for (int j = 0; j < C; ++j)
+        if (j >= n || !cat_allowed<MB>(mk, e0 + j)) bits &= ~(1u << j);
     }
+    in |= bits << (i * C);
 #pragma unroll
-    for (int j = 0; j < CAT_FEW; ++j) {
-      const unsigned w = MB == 1 ? (m[j / 4] >> (8 * (j % 4))) & 0xffu : m[MB * j / 4];
-      if (w == 0u) in &= ~(1u << j);
-    }
+    for (int j = 0; j < C; ++j) v[i * C + j] = w[j];
   }
   return in;
 }
 
-template <typename T, int MB, int G>
+template <typename T, int MB, int G, int F>
 __global__ void __launch_bounds__(256) aa_categorical_few_kernel(CatArgs a) {
   constexpr int PER = 256 / G;
   const int lane = threadIdx.x % G;
   const int64_t wanted = vt_block() * PER + threadIdx.x / G;
   // (teams past the last row stay in step with their wave on the last one and store nothing)
   const int64_t row = wanted < a.rows ? wanted : a.rows - 1;
-  float v[CAT_FEW];
-  const unsigned in = cat_few_load<T, MB>(a, row, lane * CAT_FEW, v);
-#pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i)
-    if (((in >> i) & 1u) == 0u) v[i] = -INFINITY;
+  float v[F];
+  const unsigned in = cat_few_load<T, MB, G, F>(a, row, lane, v);
   const int64_t action = cat_action(a, row);
   const float chosen = cat_action_logit<T, MB>(a, row, action);
   const float c2 = a.inv_t * CAT_LOG2E;
   CatSum u = {CAT_LOWEST, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i) u.r = fmaxf(u.r, v[i]);
+  for (int i = 0; i < F; ++i) {
+    if (((in >> i) & 1u) == 0u) v[i] = -INFINITY;
+    u.r = fmaxf(u.r, v[i]);
+  }
   u.r = wv_group_max<G>(u.r);
 #pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i) {
-    const float d = v[i] - u.r;
-    const float e = cat_exp2(d * c2);
-    u.s += e;
-    u.t = fmaf(e, fmaxf(d, CAT_LOWEST), u.t);
-  }
+  for (int i = 0; i < F; ++i) cat_add(u, v[i], c2);
   u.s = wv_group_sum<G>(u.s);
   u.t = wv_group_sum<G>(u.t);
   if (wanted >= a.rows || lane != 0) return;
@@ -645,29 +638,28 @@ __global__ void __launch_bounds__(256) aa_categorical_grad_kernel(CatGradArgs a)
 }
 
 // few actions: as the forward call, G lanes a row
-template <typename T, int MB, int G>
+template <typename T, int MB, int G, int F>
 __global__ void __launch_bounds__(256) aa_categorical_few_grad_kernel(CatGradArgs a) {
+  constexpr int C = T::C;
   const int lane = threadIdx.x % G;
   const int64_t row = vt_block() * (256 / G) + threadIdx.x / G;
   if (row >= a.f.rows) return;
-  const int e0 = lane * CAT_FEW, n = a.f.vocab - e0;
-  float v[CAT_FEW];
-  const unsigned in = cat_few_load<T, MB>(a.f, row, e0, v);
+  float v[F];
+  const unsigned in = cat_few_load<T, MB, G, F>(a.f, row, lane, v);
   const CatRow r = cat_row_grad(a, row);
-#pragma unroll
-  for (int i = 0; i < CAT_FEW; ++i) {
-    v[i] = cat_grad_one(r, v[i]) + (e0 + i == r.action ? r.hit : 0.f);
-    if (r.zero || ((in >> i) & 1u) == 0u) v[i] = 0.f;
-  }
   typename T::elem* dx = reinterpret_cast<typename T::elem*>(a.dx) +
-                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner) + e0;
+                         vt_row(row, a.f.inner, a.dx_outer, a.dx_inner);
 #pragma unroll
-  for (int i = 0; i < CAT_FEW; i += T::C) {
-    float w[T::C];
+  for (int i = 0; i < F / C; ++i) {
+    const int e0 = (i * G + lane) * C, n = a.f.vocab - e0;
+    float w[C];
 #pragma unroll
-    for (int j = 0; j < T::C; ++j) w[j] = v[i + j];
-    if (i + T::C <= n) vt_store16(dx + i, T::pack(w));
-    else vt_store_part<T>(dx + i, n - i, w);
+    for (int j = 0; j < C; ++j) {
+      w[j] = cat_grad_one(r, v[i * C + j]) + (e0 + j == r.action ? r.hit : 0.f);
+      if (r.zero || ((in >> (i * C + j)) & 1u) == 0u) w[j] = 0.f;
+    }
+    if (n >= C) vt_store16(dx + e0, T::pack(w));
+    else if (n > 0) vt_store_part<T>(dx + e0, n, w);
   }
 }
 
@@ -712,19 +704,14 @@ static CatArgs cat_args(const aa_categorical_desc* d) {
   return a;
 }
 
-// lanes that hold a row of few actions
-static int cat_few_team(int vocab) {
-  return vocab <= 8 * CAT_FEW ? 8 : vocab <= 16 * CAT_FEW ? 16 : 64;
-}
-
 template <typename T, int MB>
 static void cat_launch(const CatArgs& a, hipStream_t st) {
-  if (a.top_k == 0 && a.vocab <= 64 * CAT_FEW) {
-    const int team = cat_few_team(a.vocab);
-    const dim3 grid = vt_grid((a.rows + 256 / team - 1) / (256 / team));
-    if (team == 8) aa_categorical_few_kernel<T, MB, 8><<<grid, dim3(256), 0, st>>>(a);
-    else if (team == 16) aa_categorical_few_kernel<T, MB, 16><<<grid, dim3(256), 0, st>>>(a);
-    else aa_categorical_few_kernel<T, MB, 64><<<grid, dim3(256), 0, st>>>(a);
+  if (a.top_k == 0 && a.vocab <= CAT_FEW) {
+    const dim3 by8 = vt_grid((a.rows + 31) / 32), by16 = vt_grid((a.rows + 15) / 16), block(256);
+    if (a.vocab <= 64) aa_categorical_few_kernel<T, MB, 8, 8><<<by8, block, 0, st>>>(a);
+    else if (a.vocab <= 128) aa_categorical_few_kernel<T, MB, 16, 8><<<by16, block, 0, st>>>(a);
+    else if (a.vocab <= 256) aa_categorical_few_kernel<T, MB, 16, 16><<<by16, block, 0, st>>>(a);
+    else aa_categorical_few_kernel<T, MB, 16, 32><<<by16, block, 0, st>>>(a);
     return;
   }
   if (a.vocab <= CAT_WAVE_VOCAB) {
@@ -747,14 +734,15 @@ template <typename T, int MB>
 static void cat_launch_grad(const CatGradArgs& g, hipStream_t st) {
   const int64_t rows = g.f.rows;
   const dim3 block(256);
-  const int team = cat_few_team(g.f.vocab);
-  const dim3 few = vt_grid((rows + 256 / team - 1) / (256 / team));
-  if (team == 8)
-    aa_categorical_few_grad_kernel<T, MB, 8><<<few, block, 0, st>>>(g);
-  else if (team == 16)
-    aa_categorical_few_grad_kernel<T, MB, 16><<<few, block, 0, st>>>(g);
-  else if (g.f.vocab <= 64 * CAT_FEW)
-    aa_categorical_few_grad_kernel<T, MB, 64><<<few, block, 0, st>>>(g);
+  const dim3 by8 = vt_grid((rows + 31) / 32), by16 = vt_grid((rows + 15) / 16);
+  if (g.f.vocab <= 64)
+    aa_categorical_few_grad_kernel<T, MB, 8, 8><<<by8, block, 0, st>>>(g);
+  else if (g.f.vocab <= 128)
+    aa_categorical_few_grad_kernel<T, MB, 16, 8><<<by16, block, 0, st>>>(g);
+  else if (g.f.vocab <= 256)
+    aa_categorical_few_grad_kernel<T, MB, 16, 16><<<by16, block, 0, st>>>(g);
+  else if (g.f.vocab <= CAT_FEW)
+    aa_categorical_few_grad_kernel<T, MB, 16, 32><<<by16, block, 0, st>>>(g);
   else if (g.f.vocab <= CAT_WAVE_VOCAB)
     aa_categorical_grad_kernel<T, MB, 64><<<vt_grid((rows + 3) / 4), block, 0, st>>>(g);
   else
