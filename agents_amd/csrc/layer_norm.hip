@@ -581,7 +581,10 @@ static int64_t ln_groups(int64_t rows, int64_t width) {
   const int team = ln_bwd_team(width);
   if (team == 0) {
     // row groups of the columns' pass, 32 .. 128: f16 2000x12000 backward 86 us at 64, 71 at 128;
-    // f32 200x9000 18 at 64, 21 at 128
+    // f32 200x9000 18 at 64, 21 at 128.  Few rows: one group, which needs no launch to join it (one
+    // group | a group a row: f32 4x9001 9.2 | 11.0 us, 4x65536 20 | 29, 16x65536 23 | 34; the other
+    // way round for bf16 8x9001 13.5 | 11.8, 16x16384 15 | 12, 64x65536 68 | 42)
+    if (rows <= (width < 65536 ? 4 : 16)) return 1;
     const int64_t want = rows / 8 < 32 ? 32 : rows / 8 > 128 ? 128 : rows / 8;
     return rows < want ? rows : want;
   }
