@@ -241,7 +241,7 @@ struct CatTile {
   unsigned m[U][W];
 };
 
-// `k`: this lane's first chunk, `kb`: its wave's; chunks from k1 on read as -inf
+// `kb`: its wave's first chunk; chunks from k1 on read as -inf
 template <typename T, int MB, int U, int TEAM>
 __device__ static inline void cat_load(const typename T::elem* x, const uint8_t* mk, int kb, int lane,
                                        int k1, int skew, CatTile<T, MB, U>& t) {

@@ -7,10 +7,12 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <initializer_list>
 #include <sstream>
@@ -107,15 +109,36 @@ void same_device(const at::Tensor& t, const at::Tensor* o) {
   if (o->device() != t.device()) refuse("tensors on ", t.device().str(), " and ", o->device().str());
 }
 
+// a result's memory: no element twice (an expanded tensor), and what it reads either element for element
+// in the same place or elsewhere
+void apart(const at::Tensor& out, const at::Tensor& in, const char* name, const char* what) {
+  if (at::has_internal_overlap(out) == at::MemOverlap::Yes)
+    refuse(what, ": ", name, " must not hold an element twice (strides ", out.strides(), ")");
+  const bool same = out.data_ptr() == in.data_ptr() && out.strides() == in.strides();
+  if (!same && at::get_overlap_status(out, in) == at::MemOverlapStatus::Partial)
+    refuse(what, ": ", name, " overlaps an input without being it");
+}
+
+// a result's memory against what it must not touch at all
+void disjoint(const at::Tensor& out, std::initializer_list<const at::Tensor*> others, const char* name,
+              const char* what) {
+  for (const at::Tensor* o : others) {
+    if (o == nullptr || !o->defined()) continue;
+    const auto s = at::get_overlap_status(out, *o);
+    if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+      refuse(what, ": ", name, " overlaps another tensor of the call");
+  }
+}
+
 // ---- rows: the leading axes folded to (outer, inner) ------------------------------------------
 struct Fold {
   int64_t outer = 0, inner = 0;
 };
 
-// stride of the row index when the first `n` axes of t fold to one
-bool one_stride(const at::Tensor& t, int64_t n, int64_t* out) {
+// stride of the row index when the axes from .. to - 1 of t fold to one
+bool one_stride(const at::Tensor& t, int64_t from, int64_t to, int64_t* out) {
   int64_t stride = 0, rows = 0;
-  for (int64_t i = n - 1; i >= 0; --i) {
+  for (int64_t i = to - 1; i >= from; --i) {
     const int64_t size = t.size(i);
     if (size == 1) continue;
     if (rows == 0) {
@@ -131,28 +154,28 @@ bool one_stride(const at::Tensor& t, int64_t n, int64_t* out) {
   return true;
 }
 
-// One stride where every tensor allows it, else the last leading axis keeps one of its own (a
-// [B, T - 1] slice of [B, T] rows).  Returns `inner`.
+// One stride where every tensor allows it, else two: the leading axes are cut where both sides fold in
+// every tensor (a [B, T - 1] slice of [B, T] rows: before the last).  Returns `inner`.
 template <size_t N>
 int64_t fold_rows(int64_t lead, const std::array<const at::Tensor*, N>& ts, std::array<Fold, N>& f,
                   const char* what) {
-  bool all = true;
-  for (size_t i = 0; i < N && all; ++i) {
-    f[i] = Fold{};
-    if (ts[i] != nullptr) all = one_stride(*ts[i], lead, &f[i].outer);
+  for (int64_t cut = lead; cut == lead || cut > 0; --cut) {
+    bool all = true;
+    int64_t inner = 1;
+    for (size_t i = 0; i < N && all; ++i) {
+      f[i] = Fold{};
+      if (ts[i] == nullptr) continue;
+      all = one_stride(*ts[i], 0, cut, &f[i].outer) && one_stride(*ts[i], cut, lead, &f[i].inner);
+      inner = 1;
+      for (int64_t j = cut; j < lead; ++j) inner *= ts[i]->size(j);
+    }
+    if (all) return inner;
   }
-  if (all) return 1;
-  for (size_t i = 0; i < N; ++i) {
-    f[i] = Fold{};
-    if (ts[i] == nullptr) continue;
-    if (!one_stride(*ts[i], lead - 1, &f[i].outer))
-      refuse(what, ": leading axes of size ", ts[i]->sizes(), " with strides ", ts[i]->strides(),
-             " do not fold to two axes; pass a contiguous tensor");
-    f[i].inner = ts[i]->stride(lead - 1);
-  }
+  std::ostringstream s;
   for (size_t i = 0; i < N; ++i)
-    if (ts[i] != nullptr) return ts[i]->size(lead - 1);
-  return 1;
+    if (ts[i] != nullptr) s << " " << ts[i]->strides();
+  refuse(what, ": leading axes with strides", s.str(),
+         " do not fold to the same two axes; pass contiguous tensors");
 }
 
 int64_t rows_of(const at::Tensor& t) {
@@ -259,7 +282,7 @@ Categorical categorical_args(PyObject* logits, PyObject* actions, PyObject* mask
   c.actions = tensor(actions, what, "actions");
   const at::Tensor* m = tensor(mask, what, "mask");
   const int dtype = type_code(x);
-  if (x.dim() < 2 || dtype < 0)
+  if (x.dim() < 1 || dtype < 0)
     refuse(what, ": logits must be a float32 / bfloat16 / float16 [.., actions] tensor, got ",
            x.scalar_type(), " ", x.sizes());
   const int64_t vocab = x.size(-1);
@@ -397,6 +420,8 @@ PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse(what, ": out must be ", x.scalar_type(), " ", x.sizes(),
              " with a contiguous last axis");
     same_device(x, o);
+    apart(*o, x, "out", what);
+    disjoint(*o, {&entropy, &stats, c.actions, &c.mask, &g[0], &g[1]}, "out", what);
     out = *o;
   } else {
     out = at::empty(x.sizes(), x.options());
@@ -425,6 +450,35 @@ std::vector<const at::Tensor*> tensors(PyObject* o, PyObject** hold, const char*
   for (Py_ssize_t i = 0; i < n; ++i)
     ts[i] = &tensor_given(PySequence_Fast_GET_ITEM(*hold, i), what, name);
   return ts;
+}
+
+// results of a list: none overlaps another, and none an input other than its own
+void clip_apart(const std::vector<const void*>& src, const std::vector<void*>& dst,
+                const std::vector<int64_t>& sizes, int64_t width, const char* what) {
+  struct Range {
+    uintptr_t begin, end;
+    size_t of;
+  };
+  std::vector<Range> outs;
+  outs.reserve(dst.size());
+  for (size_t i = 0; i < dst.size(); ++i) {
+    const uintptr_t b = (uintptr_t)dst[i];
+    if (sizes[i] > 0) outs.push_back({b, b + (uintptr_t)(sizes[i] * width), i});
+  }
+  std::sort(outs.begin(), outs.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].begin < outs[i - 1].end) refuse(what, ": tensors of out overlap");
+  for (size_t i = 0; i < src.size(); ++i) {
+    const uintptr_t b = (uintptr_t)src[i], e = b + (uintptr_t)(sizes[i] * width);
+    if (b == e) continue;
+    // the first result that ends behind the input's begin
+    auto at = std::partition_point(outs.begin(), outs.end(),
+                                   [&](const Range& r) { return r.end <= b; });
+    if (at != outs.end() && at->begin < e && !(at->of == i && at->begin == b))
+      refuse(what, ": a tensor of out overlaps an input that is not its own");
+    if (at != outs.end() && at->of == i && at + 1 != outs.end() && (at + 1)->begin < e)
+      refuse(what, ": a tensor of out overlaps an input that is not its own");
+  }
 }
 
 struct Held {
@@ -474,6 +528,7 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       same_device(t0, &o);
       dst[i] = o.data_ptr();
     }
+    clip_apart(src, dst, sizes, t0.element_size(), what);
     out = out_guard.o = PySequence_List(a[4]);
     if (out == nullptr) throw Raised{};
   } else if (scale) {
@@ -544,7 +599,7 @@ void norm_stats(const at::Tensor& s, const at::Tensor& x, const char* what) {
 
 const at::Tensor& norm_input(PyObject* o, const char* what) {
   const at::Tensor& x = tensor_given(o, what, "x");
-  if (x.dim() < 2 || type_code(x) < 0 || x.size(-1) < 1)
+  if (x.dim() < 1 || type_code(x) < 0 || x.size(-1) < 1)
     refuse(what, ": x must be a float32 / bfloat16 / float16 [.., n] tensor, got ", x.scalar_type(),
            " ", x.sizes());
   norm_rows(x, "x", x, what);
@@ -566,12 +621,15 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor y, stats;
   if (const at::Tensor* o = tensor(a[4], what, "out")) {
     norm_rows(*o, "out", x, what);
+    apart(*o, x, "out", what);
+    disjoint(*o, {gamma, beta}, "out", what);
     y = *o;
   } else {
     y = at::empty(x.sizes(), x.options());
   }
   if (const at::Tensor* s = tensor(a[5], what, "stats")) {
     norm_stats(*s, x, what);
+    disjoint(*s, {&x, &y, gamma, beta}, "stats", what);
     stats = *s;
   } else {
     stats = at::empty(lead_of(x, 2), f32(x));
@@ -616,6 +674,9 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (input) {
     if (const at::Tensor* t = tensor(a[4], what, "dx")) {
       norm_rows(*t, "dx", x, what);
+      apart(*t, x, "dx", what);
+      apart(*t, dy, "dx", what);
+      disjoint(*t, {gamma, &stats}, "dx", what);
       dx = *t;
     } else {
       dx = at::empty(x.sizes(), x.options());
@@ -628,6 +689,8 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     t = tensor(a[6], what, "dbeta");
     norm_weight(t, "dbeta", x, what);
     dbeta = t != nullptr ? *t : at::empty({x.size(-1)}, f32(x));
+    disjoint(dgamma, {&dbeta, &dx, &x, &dy, gamma, &stats}, "dgamma", what);
+    disjoint(dbeta, {&dx, &x, &dy, gamma, &stats}, "dbeta", what);
   }
   const int64_t rows = rows_of(x);
   if (rows == 0) {

@@ -884,7 +884,7 @@ def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dent
     """d loss / d logits from d loss / d log_prob and d loss / d entropy ([..] float32, either may be
     None); `forward` is what categorical_log_prob returned for the same logits, actions, mask,
     temperature and first_action.  Masked actions and padding rows get 0.  The result has the logits'
-    type; `out` may be the logits' own tensor."""
+    type; `out` may be the logits' own tensor (else it must not overlap them)."""
     return (_token_ops or _bind()).categorical_log_prob_backward(
         logits, actions, forward.entropy, forward.stats, dlog_prob, dentropy, mask, temperature,
         first_action, out)
@@ -894,9 +894,10 @@ def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dent
 def clip_by_global_norm(tensors, clip_norm, out=None):
     """tf.clip_by_global_norm: ([t * clip_norm / max(global norm, clip_norm)], global norm) of a list
     of contiguous float32 / bfloat16 / float16 tensors of one type (csrc/grad_clip.hip).  `out`: a
-    list that receives the clipped tensors, `tensors` itself for clipping in place; without it they
-    are pieces of one new allocation.  The norm is a float32 scalar on the device; one that is not
-    finite makes every clipped value NaN."""
+    list that receives the clipped tensors, `tensors` itself for clipping in place (no result may
+    overlap another, or an input other than its own); without it they are pieces of one new
+    allocation.  The norm is a float32 scalar on the device; one that is not finite makes every
+    clipped value NaN."""
     return (_token_ops or _bind()).clip(tensors, clip_norm, False, True, out, "clip_by_global_norm")
 
 

@@ -223,6 +223,34 @@ def test_strides(dev):
     check(same, a8, None, 1.0, 0, ops.categorical_log_prob(same, a8))
 
 
+def test_one_row_without_leading_axes(dev):
+    logits = torch.randn(700, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    action = torch.tensor(9, device=dev)
+    mask = torch.ones(700, dtype=torch.bool, device=dev)
+    r = ops.categorical_log_prob(logits, action, mask=mask, top_k=3)
+    assert r.log_prob.shape == () and r.top_ids.shape == (3,)
+    check(logits[None], action[None], mask[None], 1.0, 3, r)
+    g = torch.tensor(2.0, device=dev)
+    d = ops.categorical_log_prob_backward(logits, action, r, g, mask=mask)
+    check_grad(logits[None], action[None], mask[None], 1.0, g[None], None, d)
+
+
+def test_results_over_inputs_are_refused(dev):
+    buf = torch.randn(4, 20, device=dev)
+    logits, actions = buf[:, :10], torch.zeros(4, dtype=torch.int64, device=dev)
+    r = ops.categorical_log_prob(logits, actions)
+    g = torch.ones(4, device=dev)
+    with pytest.raises(ValueError, match="twice"):
+        ops.categorical_log_prob_backward(logits, actions, r, g,
+                                          out=torch.zeros(1, 10, device=dev).expand(4, 10))
+    flat = torch.randn(100, device=dev)
+    logits = flat[:40].view(4, 10)
+    r = ops.categorical_log_prob(logits, actions)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.categorical_log_prob_backward(logits, actions, r, g, out=flat[5:45].view(4, 10))
+    ops.categorical_log_prob_backward(logits, actions, r, g, out=flat[40:80].view(4, 10))
+
+
 def test_in_place_gradient(dev):
     for dtype, V in ((torch.float32, 37), (torch.bfloat16, 5001)):
         logits, actions, _, g, h = inputs((6, V), dtype, None, dev, 11)

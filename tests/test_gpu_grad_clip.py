@@ -97,6 +97,20 @@ def test_in_place(dev):
         assert torch.equal(a, b)
 
 
+def test_results_over_other_tensors_are_refused(dev):
+    flat = torch.randn(100, device=dev)
+    a, b, c = flat[:30], flat[30:60], flat[60:90]
+    for ts, outs in (([a, b], [b, a]), ([a, a], [a, a]), ([a, b], [c, flat[70:100]]),
+                     ([a], [flat[1:31]]), ([flat[:30], flat[40:70]], [flat[:30], flat[20:50]])):
+        for f in (ops.clip_by_global_norm, ops.clip_by_norms):
+            with pytest.raises(ValueError, match="overlap"):
+                f(ts, 1.0, out=outs)
+    want, norm = ops.clip_by_global_norm([a, a, b], 1.0)         # read twice: counted twice
+    got, n2 = ops.clip_by_global_norm([a.clone(), a.clone(), b.clone()], 1.0)
+    assert torch.equal(norm, n2) and all(torch.equal(p, q) for p, q in zip(want, got))
+    ops.clip_by_global_norm([a, b], 1.0, out=[a, c])
+
+
 def test_unclipped_values_are_the_same_bits(dev):
     ts = grads(SETS["odd"], torch.bfloat16, dev, 6)
     got, norm = ops.clip_by_global_norm(ts, 1e4)

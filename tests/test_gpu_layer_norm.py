@@ -182,6 +182,61 @@ def test_strides_and_in_place(dev):
                 assert torch.equal(p, q)
 
 
+def test_one_row_without_leading_axes(dev):
+    x, dy, gamma, beta = inputs((1, 90), torch.float32, dev, 5)
+    y, stats = ops.layer_norm_forward(x[0], gamma, beta)
+    assert y.shape == (90,) and stats.shape == (2,)
+    check_forward(x, gamma, beta, 1e-3, y[None], stats[None])
+    dx, dg, db = ops.layer_norm_backward(dy[0], x[0], gamma, stats)
+    check_backward(dy, x, gamma, 1e-3, (dx[None], dg, db))
+
+
+def test_results_over_inputs_are_refused(dev):
+    flat = torch.randn(100, device=dev)
+    x, w = flat[:40].view(4, 10), torch.ones(10, device=dev)
+    y, stats = ops.layer_norm_forward(x, w, None)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.layer_norm_forward(x, w, None, out=flat[5:45].view(4, 10))
+    with pytest.raises(ValueError, match="twice"):
+        ops.layer_norm_forward(x, w, None, out=torch.zeros(10, device=dev).expand(4, 10))
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.layer_norm_backward(y, x, w, stats, dx=flat[5:45].view(4, 10))
+    for bad in (dict(dgamma=flat[80:90], dbeta=flat[85:95]), dict(dgamma=w), dict(dgamma=flat[:10])):
+        with pytest.raises(ValueError, match="dgamma overlaps"):
+            ops.layer_norm_backward(y, x, w, stats, **bad)
+
+
+@pytest.mark.parametrize("cut", ["before the last", "before the last two", "an axis of one"])
+def test_leading_axes_that_fold_to_two(dev, cut):
+    x, dy, gamma, beta = inputs((3, 5, 4, 33), torch.float32, dev, 8)
+    if cut == "before the last":
+        x, dy = x[:, :, :3], dy[:, :, :3]
+    elif cut == "before the last two":
+        x, dy = x[:, :4], dy[:, :4]
+    else:
+        x, dy = x[:, :4, :1], dy[:, :4, :1]
+    y, stats = ops.layer_norm_forward(x, gamma, beta)
+    same, st = ops.layer_norm_forward(x.contiguous(), gamma, beta)
+    assert torch.equal(y, same) and torch.equal(stats, st)
+    got = ops.layer_norm_backward(dy, x, gamma, stats)
+    want = ops.layer_norm_backward(dy.contiguous(), x.contiguous(), gamma, stats)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_leading_axes_that_do_not_fold(dev):
+    x, _, gamma, beta = inputs((3, 5, 4, 33), torch.float32, dev, 8)
+    with pytest.raises(ValueError, match="two axes"):
+        ops.layer_norm_forward(x[:, :4, :3], gamma, beta)
+
+
+@pytest.mark.parametrize("rows,width", [(1, 9001), (4, 9001), (5, 9001), (16, 65536), (17, 65537)])
+def test_few_wide_rows(dev, rows, width):
+    x, dy, gamma, beta = inputs((rows, width), torch.bfloat16, dev, rows)
+    y, stats = ops.layer_norm_forward(x, gamma, beta)
+    check_forward(x, gamma, beta, 1e-3, y, stats)
+    check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
+
+
 def test_no_rows(dev):
     x = torch.empty(0, 5, device=dev)
     y, stats = ops.layer_norm_forward(x, None, None)
