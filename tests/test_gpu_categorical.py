@@ -119,6 +119,32 @@ def test_values_and_gradient(dev, shape, dtype, mask_kind):
         check_grad(logits, actions, mask, t, gg, hh, d)
 
 
+@pytest.mark.parametrize("vocab", [8, 9, 63, 127, 128, 129, 200, 256, 257, 300, 511, 512, 513])
+@pytest.mark.parametrize("rows", [1, 15, 33])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask_kind", [None, torch.bool, torch.int32])
+def test_few_actions(dev, vocab, rows, dtype, mask_kind):
+    """Around the sizes at which a row's team changes, rows at every alignment."""
+    logits, actions, mask, g, h = inputs((rows, vocab + 1), dtype, mask_kind, dev, vocab)
+    logits, actions = logits[:, 1:], actions.clamp(max=vocab - 1)
+    mask = None if mask is None else mask[:, 1:]
+    r = ops.categorical_log_prob(logits, actions, mask=mask)
+    check(logits, actions, mask, 1.0, 0, r)
+    d = ops.categorical_log_prob_backward(logits, actions, r, g, h, mask=mask)
+    check_grad(logits, actions, mask, 1.0, g, h, d)
+
+
+@pytest.mark.parametrize("shape", [(9, 18), (33, 700), (5, 5003), (1, 60001), (300, 20011)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask_kind", [torch.bool, torch.int32])
+def test_alternatives_under_masks(dev, shape, dtype, mask_kind):
+    logits, actions, mask, _, _ = inputs(shape[:1] + (shape[1] + 3,), dtype, mask_kind, dev, 31)
+    logits, mask, actions = logits[:, 3:], mask[:, 3:], actions.clamp(max=shape[1] - 1)
+    for k in (1, 11):
+        r = ops.categorical_log_prob(logits, actions, mask=mask, top_k=k)
+        check(logits, actions, mask, 1.0, k, r)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 700])
 @pytest.mark.parametrize("vocab,top_k", [(2, 2), (7, 64), (300, 5), (4096, 20), (4099, 64), (40003, 1),
                                          (131072, 20)])
@@ -147,6 +173,16 @@ def test_alternatives_of_ordered_rows(dev, order, vocab):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("vocab", [6, 5000, 40001])
 def test_corners(dev, dtype, vocab):
+    corners(dev, dtype, vocab, 4)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [6, 60, 100, 200, 300, 600, 5000, 40001])
+def test_corners_without_alternatives(dev, dtype, vocab):
+    corners(dev, dtype, vocab, 0)
+
+
+def corners(dev, dtype, vocab, top_k):
     """Empty masks, the type's lowest value, infinities and NaN in masked and in allowed places, an
     action that its mask excludes, one past the end, padding."""
     inf, nan, low = float("inf"), float("nan"), torch.finfo(dtype).min
@@ -169,8 +205,8 @@ def test_corners(dev, dtype, vocab):
     actions[12] = -7                                  # padding; its logits are not used
     logits[12] = nan
     logits[13, 0] = -inf                              # the action's logit is -inf
-    r = ops.categorical_log_prob(logits, actions, mask=mask, top_k=4)
-    check(logits, actions, mask, 1.0, 4, r)
+    r = ops.categorical_log_prob(logits, actions, mask=mask, top_k=top_k)
+    check(logits, actions, mask, 1.0, top_k, r)
     g = torch.linspace(-1, 1, n, device=dev)
     h = torch.linspace(0.5, -0.5, n, device=dev)
     d = ops.categorical_log_prob_backward(logits, actions, r, g, h, mask=mask)
@@ -292,6 +328,24 @@ def test_many_rows(dev):
     d = ops.categorical_log_prob_backward(logits, actions, r, g)
     hot = torch.nn.functional.one_hot(actions, V)
     assert (d.double() - (hot - want.exp())).abs().max() < 64 * U
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_gradients(dev, dtype):
+    """Gradients that are stored past the caches are those of a part of the rows, bit for bit."""
+    V = 33001
+    rows = (140 << 20) // (V * dtype.itemsize)
+    gen = torch.Generator(device=dev).manual_seed(4)
+    logits = torch.randn(rows, V, generator=gen, device=dev).to(dtype)
+    actions = torch.randint(0, V, (rows,), generator=gen, device=dev)
+    g = torch.randn(rows, generator=gen, device=dev)
+    r = ops.categorical_log_prob(logits, actions)
+    d = ops.categorical_log_prob_backward(logits, actions, r, g, g)
+    cut = slice(rows - 5, rows)
+    part = type(r)(r.log_prob[cut], r.entropy[cut], None, None, r.stats[cut])
+    want = ops.categorical_log_prob_backward(logits[cut], actions[cut], part, g[cut], g[cut])
+    assert torch.equal(d[cut], want)
+    check_grad(logits[cut], actions[cut], None, 1.0, g[cut], g[cut], want)
 
 
 def test_offsets_past_32_bits(dev):

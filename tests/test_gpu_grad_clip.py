@@ -88,6 +88,28 @@ def test_large_and_unaligned(dev):
             (out[29_000_002:29_000_010] == 3).all() and (out[29_001_010:] == 3).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_past_the_caches(dev, dtype):
+    """A list whose results are stored past the caches, at odd addresses."""
+    n = (260 << 20) // dtype.itemsize + 77
+    flat = (torch.randn(n + 9, device=dev, generator=torch.Generator(device=dev).manual_seed(7))
+            * 0.01).to(dtype)
+    ts = [flat[1:n // 3], flat[n // 3:n // 3 + 5], flat[n // 3 + 5:n + 2]]
+    norm = sum((t.double() ** 2).sum() for t in ts).sqrt()
+    out = torch.full_like(flat, 3.0)
+    outs = [out[3:n // 3 + 2], out[n // 3 + 2:n // 3 + 7], out[n // 3 + 7:n + 4]]
+    _, got = ops.clip_by_global_norm(ts, 2.0, out=outs)
+    # the factor and its product are rounded to fp32, the result to its type (fp16: or to half of its
+    # smallest spacing)
+    half = torch.finfo(dtype).eps / 2
+    assert abs(float(got) - float(norm)) <= 2 * U * float(norm)
+    for t, o in zip(ts, outs):
+        want = t.double() * (2.0 / norm)
+        tol = want.abs() * (half + 3 * U) + (2.0 ** -25 if dtype == torch.float16 else 1e-40)
+        assert bool(((o.double() - want).abs() <= tol).all())
+    assert (out[:3] == 3).all() and (out[n + 4:] == 3).all()
+
+
 def test_in_place(dev):
     ts = grads(SETS["odd"], torch.float32, dev, 5)
     want, norm = ops.clip_by_global_norm(ts, 0.3)

@@ -113,6 +113,17 @@ def test_forward_backward(dev, shape, dtype):
     check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
 
 
+@pytest.mark.parametrize("shape", [(70000, 20), (30000, 65), (9000, 300), (5000, 1003), (2100, 4096),
+                                   (1100, 8192), (300, 16384)])
+def test_several_rows_a_team(dev, shape):
+    """More rows than the launch has teams, in both directions, the last round not full."""
+    dtype = torch.float32 if shape[0] % 1000 else torch.bfloat16
+    x, dy, gamma, beta = inputs(shape, dtype, dev, 6)
+    y, stats = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    check_forward(x, gamma, beta, 1e-3, y, stats)
+    check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
+
+
 @pytest.mark.parametrize("shape", [(9, 130), (5, 5000), (3, 20000)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_without_weights_masks_parts(dev, shape, dtype):

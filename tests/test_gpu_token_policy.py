@@ -70,6 +70,12 @@ STACKS = {
     "conv": ((8, 8, 4), lambda: [L.Conv2D(16, 3, 1, "tanh"), L.LayerNormalization(),
                                  L.Conv2D(12, 2, 2, "tanh"), L.LayerNormalization(), L.Flatten(),
                                  L.Dense(40, "tanh"), L.LayerNormalization(), L.Dense(5)]),
+    "conv-flat": ((9, 9, 4), lambda: [L.Conv2D(16, 3, 2, "tanh"), L.Flatten(), L.LayerNormalization(),
+                                      L.Dense(40, "tanh"), L.Dense(5)]),
+    "conv-unflattened": ((9, 9, 4), lambda: [L.Conv2D(16, 3, 2, "tanh"), L.LayerNormalization(),
+                                             L.Dense(5)]),
+    "before-conv": ((9, 9, 4), lambda: [L.LayerNormalization(), L.Conv2D(16, 3, 1, "tanh"),
+                                        L.Conv2D(16, 3, 1, "tanh"), L.Flatten(), L.Dense(5)]),
 }
 
 
@@ -97,7 +103,7 @@ def test_sequential_with_layer_normalization(dev, name, side):
     dout = torch.randn(want.shape, generator=torch.Generator().manual_seed(2))
     (want * dout.double()).sum().backward()
     stream = ops.new_side_stream(dev) if side else None
-    dense_first = name != "conv"
+    dense_first = not name.startswith("conv")
     dx = torch.zeros(B, *shape, device=dev) if dense_first else None
     net.backward(dout.to(dev), slot="t", side_stream=stream, input_grad=dx)
     torch.cuda.synchronize()
