@@ -113,6 +113,15 @@ def test_forward_backward(dev, shape, dtype):
     check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
 
 
+@pytest.mark.parametrize("shape", [(129, 64), (256, 60), (257, 64), (64, 250), (65, 250), (32, 512), (33, 512),
+                                   (16, 1000), (17, 1000), (4, 4096), (5, 4096), (2, 8192), (3, 8000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_around_two_rounds_of_a_workgroup(dev, shape, dtype):
+    x, dy, gamma, beta = inputs(shape, dtype, dev, 12)
+    y, stats = ops.layer_norm_forward(x, gamma, beta, 1e-3)
+    check_backward(dy, x, gamma, 1e-3, ops.layer_norm_backward(dy, x, gamma, stats))
+
+
 @pytest.mark.parametrize("shape", [(70000, 20), (30000, 65), (9000, 300), (5000, 1003), (2100, 4096),
                                    (1100, 8192), (300, 16384)])
 def test_several_rows_a_team(dev, shape):
