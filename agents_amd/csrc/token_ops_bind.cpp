@@ -568,13 +568,16 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     out = out_guard.o = Py_None;
     Py_INCREF(out);
   }
-  const at::Tensor norm = each ? at::empty({(int64_t)n}, f32(t0)) : at::empty({}, f32(t0));
+  // (the scratch, some kilobytes of sums, behind the norms)
   const int64_t need = lib.clip_bytes(sizes.data(), (int32_t)n);
-  const at::Tensor ws = scratch(need, t0);
+  const int64_t norms = each ? (int64_t)n : 1;
+  Pieces small(Pieces::room(norms, 4) + (need + 3) / 4, f32(t0));
+  const at::Tensor norm = each ? small.take({norms}) : small.take({});
+  void* const ws = static_cast<float*>(small.flat.data_ptr()) + small.at;
   {
     OnDevice on(t0);
     check(unlocked(lib.clip, src.data(), scale ? dst.data() : nullptr, sizes.data(), (int32_t)n,
-                   dtype, clip, (int32_t)each, (float*)norm.data_ptr(), data(ws), need, on.stream),
+                   dtype, clip, (int32_t)each, (float*)norm.data_ptr(), ws, need, on.stream),
           "aa_clip_tensors");
   }
   Held wrapped;
