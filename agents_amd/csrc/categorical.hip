@@ -14,7 +14,7 @@
 // which reads and writes them, 82 .. 84 us, 6.4 TB/s; f16 2044x50001, 204 MB, 42 .. 45 and 64 .. 66),
 // by launch and latency for a few actions (f32 4096x18 with an int32 mask: 3.7 and 3.9 us).  Few rows:
 // a row is split over workgroups and the parts joined by a second launch (bf16 1x131072 with 20
-// alternatives: 8.5 + 5 us).
+// alternatives: 8.5 + 4 us).
 #include <math.h>
 #include "common.h"
 #include "agents_amd.h"
