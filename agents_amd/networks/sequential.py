@@ -953,15 +953,19 @@ class Sequential(network.Network):
                 dx_prep_pending = self._hoist_dx_prep(s, B, hi, lo, fork_event=prep_fork)
                 prep_fork = None
 
-        side_used = False
+        forked = False     # the side stream waits for main in this range
+
+        def fork_side():
+            nonlocal forked
+            if side_stream is not main:
+                forked = True
+                side_stream.wait_stream(main)
 
         def on_side(fn, fork=True):
-            nonlocal side_used
             if side_stream is main:
                 return fn()
-            side_used = True
             if fork:
-                side_stream.wait_stream(main)  # dZ of this layer is ready once main gets here
+                fork_side()        # dZ of this layer is ready once main gets here
             with ops.side_line(side_stream):
                 return fn()
 
@@ -996,8 +1000,8 @@ class Sequential(network.Network):
                               and ops.dense_small_backward_ok(x, dz2, x if prev_act else None))
                 if fused_head:
                     # the head's input and weight gradients in one launch (both a few us)
-                    if DX_FIRST and side_stream is not main:
-                        side_stream.wait_stream(main)
+                    if DX_FIRST:
+                        fork_side()
                     ops.dense_small_backward(x, dz2, self._kviews[i], s.dxs[i].view(B, -1),
                                              self._gkviews[i], mask_src=x if prev_act else None,
                                              mask_act=prev_act, bias_grad=self._gbviews[i])
@@ -1007,7 +1011,7 @@ class Sequential(network.Network):
                 if i > 0:
                     dx = s.dxs[i].view(B, -1)
                     if DX_FIRST:
-                        side_stream.wait_stream(main) if side_stream is not main else None
+                        fork_side()
                     ops.dense_dx(dz2, self._kviews[i], dx, mask_src=x if prev_act else None,
                                  mask_act=prev_act)
                     issue_late_prep()
@@ -1044,7 +1048,7 @@ class Sequential(network.Network):
                 if i > 0:
                     issue_late_prep()
                     if DX_FIRST:
-                        side_stream.wait_stream(main) if side_stream is not main else None
+                        fork_side()
                     prepared = s.dx_prep.get(i) if (s.dx_prep and HOIST_PREP) else None
                     if pw_dx is not None:
                         prepared = pw_dx.get(i)
@@ -1079,9 +1083,10 @@ class Sequential(network.Network):
             self._pending_keep = pending_dw          # backward_resume continues this list
         elif keep:
             self._grad_slabs = ops.grad_slabs(pending_dw, self.flat_grads)
-        if side_stream is not main and (side_used or lo > 0 or hi > lo):
-            # (a resumed range of layer 0 alone with its weight gradient on main has not touched
-            # the side stream: nothing to join -- and under capture nothing that could be joined)
+        if forked:
+            # (a range that has not forked the side stream -- layer 0 alone with its weight gradient
+            # on main, normalisations above it -- has nothing to join, and under capture nothing that
+            # could be joined: a wait for a stream outside the capture ends it)
             main.wait_stream(side_stream)
 
     def _first_div(self):
