@@ -100,13 +100,20 @@ int type_code(const at::Tensor& t) {
   }
 }
 
-void same_device(const at::Tensor& t, const at::Tensor* o) {
-  if (o == nullptr) return;
-  if (!o->is_cuda())
-    raise(lib_error,
-          "agents_amd kernels need device tensors (torch 'cuda' = HIP on ROCm); got a ",
-          o->device().str(), " tensor.  There is no CPU fallback on the product path.");
-  if (o->device() != t.device()) refuse("tensors on ", t.device().str(), " and ", o->device().str());
+// The last check of a call, behind all that look at types, shapes and layouts: those hold for host tensors
+// as well, so that their refusals are tested without a device.
+void on_device(std::initializer_list<const at::Tensor*> ts) {
+  const at::Tensor* first = nullptr;
+  for (const at::Tensor* t : ts) {
+    if (t == nullptr || !t->defined()) continue;
+    if (!t->is_cuda())
+      raise(lib_error,
+            "agents_amd kernels need device tensors (torch 'cuda' = HIP on ROCm); got a ",
+            t->device().str(), " tensor.  There is no CPU fallback on the product path.");
+    if (first == nullptr) first = t;
+    if (t->device() != first->device())
+      refuse("tensors on ", first->device().str(), " and ", t->device().str());
+  }
 }
 
 // a result's memory: no element twice (an expanded tensor), and what it reads either element for element
@@ -182,6 +189,12 @@ int64_t rows_of(const at::Tensor& t) {
   int64_t n = 1;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
   return n;
+}
+
+// a contiguous tensor of t's sizes, its rows folded with `inner`
+Fold own_fold(const at::Tensor& t, int64_t inner) {
+  const int64_t width = t.size(-1);
+  return inner == 1 ? Fold{width, 0} : Fold{inner * width, width};
 }
 
 bool last_contiguous(const at::Tensor& t) {
@@ -333,9 +346,6 @@ Categorical categorical_args(PyObject* logits, PyObject* actions, PyObject* mask
     }
     if (!last_contiguous(c.mask)) refuse(what, ": the last axis of mask must be contiguous");
   }
-  same_device(x, &x);
-  same_device(x, c.actions);
-  if (c.mask.defined()) same_device(x, &c.mask);
   aa_categorical_desc& d = c.d;
   d = aa_categorical_desc{};
   d.rows = rows_of(x);
@@ -376,6 +386,7 @@ PyObject* py_categorical(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (k > c.d.vocab) k = c.d.vocab;
   categorical_fold(c, nullptr, what);
   const at::Tensor& x = *c.logits;
+  on_device({&x, c.actions, &c.mask});
   const auto lead = lead_of(x);
   at::Tensor log_prob, ids, top;
   const int64_t rows = c.d.rows;
@@ -424,7 +435,6 @@ PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (t->scalar_type() != at::kFloat || t->sizes() != at::IntArrayRef(lead))
       refuse(what, ": ", name, " must be float32 ", at::IntArrayRef(lead), ", got ",
              t->scalar_type(), " ", t->sizes());
-    same_device(x, t);
     g[i] = t->contiguous();
   }
   const auto lead2 = lead_of(x, 2);
@@ -434,22 +444,23 @@ PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (stats.sizes() != at::IntArrayRef(lead2) || stats.scalar_type() != at::kFloat ||
       !stats.is_contiguous())
     refuse(what, ": forward.stats is not of these logits");
-  same_device(x, &entropy);
-  same_device(x, &stats);
   at::Tensor out;
-  if (const at::Tensor* o = tensor(a[9], what, "out")) {
+  const at::Tensor* const o = tensor(a[9], what, "out");
+  if (o != nullptr) {
     if (o->scalar_type() != x.scalar_type() || o->sizes() != x.sizes() || !last_contiguous(*o))
       refuse(what, ": out must be ", x.scalar_type(), " ", x.sizes(),
              " with a contiguous last axis");
-    same_device(x, o);
     apart(*o, x, "out", what);
     disjoint(*o, {&entropy, &stats, c.actions, &c.mask, &g[0], &g[1]}, "out", what);
     out = *o;
-  } else {
+  }
+  Fold f = categorical_fold(c, o, what);
+  on_device({&x, c.actions, &c.mask, &entropy, &stats, &g[0], &g[1], &out});
+  if (!out.defined()) {
     out = at::empty(x.sizes(), x.options());
+    f = own_fold(x, c.d.inner);
   }
   if (c.d.rows > 0) {
-    const Fold f = categorical_fold(c, &out, what);
     c.d.entropy = (float*)data(entropy);
     c.d.stats = (float*)data(stats);
     OnDevice on(x);
@@ -534,23 +545,25 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (t.scalar_type() != t0.scalar_type() || !t.is_contiguous())
       refuse(what, ": tensors must be contiguous and of one type, got ", t.scalar_type(), " ",
              t.sizes(), " strides ", t.strides(), " beside ", t0.scalar_type());
-    same_device(t0, &t);
     src[i] = t.data_ptr();
     sizes[i] = t.numel();
   }
-  PyObject* out = nullptr;     // owned; released on every way out but the last
-  Held out_guard;
+  std::vector<const at::Tensor*> os;
   if (scale && a[4] != Py_None) {
-    const std::vector<const at::Tensor*> os = tensors(a[4], &hold_out.o, what, "out");
+    os = tensors(a[4], &hold_out.o, what, "out");
     if (os.size() != n) refuse(what, ": out must mirror the tensors");
     for (size_t i = 0; i < n; ++i) {
       const at::Tensor& o = *os[i];
       if (o.scalar_type() != t0.scalar_type() || o.sizes() != ts[i]->sizes() || !o.is_contiguous())
         refuse(what, ": out must mirror the tensors");
-      same_device(t0, &o);
       dst[i] = o.data_ptr();
     }
     clip_apart(src, dst, sizes, t0.element_size(), what);
+  }
+  for (size_t i = 0; i < n; ++i) on_device({&t0, ts[i], os.empty() ? nullptr : os[i]});
+  PyObject* out = nullptr;     // owned; released on every way out but the last
+  Held out_guard;
+  if (!os.empty()) {
     out = out_guard.o = PySequence_List(a[4]);
     if (out == nullptr) throw Raised{};
   } else if (scale) {
@@ -594,7 +607,6 @@ void norm_rows(const at::Tensor& t, const char* name, const at::Tensor& x, const
     refuse(what, ": ", name, " must be ", x.scalar_type(), " ", x.sizes(),
            " with a contiguous last axis, got ", t.scalar_type(), " ", t.sizes(), " strides ",
            t.strides());
-  same_device(x, &t);
 }
 
 void norm_weight(const at::Tensor* w, const char* name, const at::Tensor& x, const char* what) {
@@ -603,14 +615,12 @@ void norm_weight(const at::Tensor* w, const char* name, const at::Tensor& x, con
       !w->is_contiguous())
     refuse(what, ": ", name, " must be contiguous float32 [", x.size(-1), "], got ",
            w->scalar_type(), " ", w->sizes());
-  same_device(x, w);
 }
 
 void norm_stats(const at::Tensor& s, const at::Tensor& x, const char* what) {
   const auto want = lead_of(x, 2);
   if (s.sizes() != at::IntArrayRef(want) || s.scalar_type() != at::kFloat || !s.is_contiguous())
     refuse(what, ": stats must be contiguous float32 ", at::IntArrayRef(want));
-  same_device(x, &s);
 }
 
 const at::Tensor& norm_input(PyObject* o, const char* what) {
@@ -635,26 +645,31 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double epsilon = number(a[3], what, "epsilon");
   if (!(epsilon >= 0)) refuse(what, ": epsilon must not be negative, got ", epsilon);
   at::Tensor y, stats;
-  if (const at::Tensor* o = tensor(a[4], what, "out")) {
-    norm_rows(*o, "out", x, what);
-    apart(*o, x, "out", what);
-    disjoint(*o, {gamma, beta}, "out", what);
-    y = *o;
-  } else {
-    y = at::empty(x.sizes(), x.options());
+  const at::Tensor* const out = tensor(a[4], what, "out");
+  if (out != nullptr) {
+    norm_rows(*out, "out", x, what);
+    apart(*out, x, "out", what);
+    disjoint(*out, {gamma, beta}, "out", what);
+    y = *out;
   }
   if (const at::Tensor* s = tensor(a[5], what, "stats")) {
     norm_stats(*s, x, what);
     disjoint(*s, {&x, &y, gamma, beta}, "stats", what);
     stats = *s;
-  } else {
-    stats = at::empty(lead_of(x, 2), f32(x));
   }
   const int64_t rows = rows_of(x);
+  // (results of the call's own are contiguous: they fold as x does)
+  std::array<Fold, 2> f;
+  const int64_t inner = rows > 0 ? fold_rows<2>(x.dim() - 1, {&x, out}, f, what) : 1;
+  on_device({&x, gamma, beta, &y, &stats});
+  if (!y.defined()) {
+    y = at::empty(x.sizes(), x.options());
+    f[1] = own_fold(x, inner);
+  }
+  if (!stats.defined()) stats = at::empty(lead_of(x, 2), f32(x));
   if (rows > 0) {
     aa_layer_norm_desc d{};
-    std::array<Fold, 2> f;
-    d.inner = fold_rows<2>(x.dim() - 1, {&x, &y}, f, what);
+    d.inner = inner;
     d.rows = rows;
     d.width = x.size(-1);
     d.x = x.data_ptr(); d.x_outer = f[0].outer; d.x_inner = f[0].inner;
@@ -687,34 +702,38 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool params = a[8] == Py_True, input = a[9] == Py_True;
   if (!params && !input) refuse(what, ": nothing to compute");
   at::Tensor dx, dgamma, dbeta;
-  if (input) {
-    if (const at::Tensor* t = tensor(a[4], what, "dx")) {
-      norm_rows(*t, "dx", x, what);
-      apart(*t, x, "dx", what);
-      apart(*t, dy, "dx", what);
-      disjoint(*t, {gamma, &stats}, "dx", what);
-      dx = *t;
-    } else {
-      dx = at::empty(x.sizes(), x.options());
-    }
+  const at::Tensor* const dx_out = input ? tensor(a[4], what, "dx") : nullptr;
+  if (dx_out != nullptr) {
+    norm_rows(*dx_out, "dx", x, what);
+    apart(*dx_out, x, "dx", what);
+    apart(*dx_out, dy, "dx", what);
+    disjoint(*dx_out, {gamma, &stats}, "dx", what);
+    dx = *dx_out;
   }
   if (params) {
     const at::Tensor* g = tensor(a[5], what, "dgamma");
     const at::Tensor* b = tensor(a[6], what, "dbeta");
     norm_weight(g, "dgamma", x, what);
     norm_weight(b, "dbeta", x, what);
-    if (g == nullptr || b == nullptr) {
-      Pieces pieces(((g == nullptr) + (b == nullptr)) * Pieces::room(x.size(-1), 4), f32(x));
-      dgamma = g != nullptr ? *g : pieces.take({x.size(-1)});
-      dbeta = b != nullptr ? *b : pieces.take({x.size(-1)});
-    } else {
-      dgamma = *g;
-      dbeta = *b;
-    }
-    disjoint(dgamma, {&dbeta, &dx, &x, &dy, gamma, &stats}, "dgamma", what);
-    disjoint(dbeta, {&dx, &x, &dy, gamma, &stats}, "dbeta", what);
+    if (g != nullptr) disjoint(*g, {b, &dx, &x, &dy, gamma, &stats}, "dgamma", what);
+    if (b != nullptr) disjoint(*b, {&dx, &x, &dy, gamma, &stats}, "dbeta", what);
+    if (g != nullptr) dgamma = *g;
+    if (b != nullptr) dbeta = *b;
   }
+  const int32_t mask_act = (int32_t)whole(a[7], what, "mask_act");
   const int64_t rows = rows_of(x);
+  std::array<Fold, 3> f;
+  const int64_t inner = rows > 0 ? fold_rows<3>(x.dim() - 1, {&x, &dy, dx_out}, f, what) : 1;
+  on_device({&x, &dy, gamma, &stats, &dx, &dgamma, &dbeta});
+  if (input && !dx.defined()) {
+    dx = at::empty(x.sizes(), x.options());
+    f[2] = own_fold(x, inner);
+  }
+  if (params && (!dgamma.defined() || !dbeta.defined())) {
+    Pieces pieces((!dgamma.defined() + !dbeta.defined()) * Pieces::room(x.size(-1), 4), f32(x));
+    if (!dgamma.defined()) dgamma = pieces.take({x.size(-1)});
+    if (!dbeta.defined()) dbeta = pieces.take({x.size(-1)});
+  }
   if (rows == 0) {
     if (params) {
       dgamma.zero_();
@@ -722,8 +741,7 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
   } else {
     aa_layer_norm_desc d{};
-    std::array<Fold, 3> f;
-    d.inner = fold_rows<3>(x.dim() - 1, {&x, &dy, input ? &dx : nullptr}, f, what);
+    d.inner = inner;
     d.rows = rows;
     d.width = x.size(-1);
     d.x = x.data_ptr(); d.x_outer = f[0].outer; d.x_inner = f[0].inner;
@@ -734,7 +752,7 @@ PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     d.dgamma = (float*)data(dgamma);
     d.dbeta = (float*)data(dbeta);
     d.dtype = type_code(x);
-    d.mask_act = (int32_t)whole(a[7], what, "mask_act");
+    d.mask_act = mask_act;
     const int64_t need = lib.norm_bytes(&d);
     const at::Tensor ws = scratch(need, x);
     OnDevice on(x);
