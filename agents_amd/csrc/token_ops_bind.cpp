@@ -7,7 +7,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -116,25 +115,114 @@ void on_device(std::initializer_list<const at::Tensor*> ts) {
   }
 }
 
-// a result's memory: no element twice (an expanded tensor), and what it reads either element for element
-// in the same place or elsewhere
+// ---- memory: what a result may share with the other tensors of a call -----------------------------
+// A tensor as runs of `width` bytes, one for every choice of multiples of its axes' strides.
+struct Runs {
+  struct Axis {
+    int64_t stride, size;          // bytes, multiples
+  };
+  uintptr_t begin = 0;
+  int64_t width = 0, reach = 0;    // bytes of a run; from the first run's begin to the last one's
+  bool twice = false;              // an axis of stride 0
+  c10::SmallVector<Axis, 6> axes;
+  explicit Runs(const at::Tensor& t) {
+    if (t.numel() == 0) return;    // (width 0: meets nothing)
+    begin = (uintptr_t)t.data_ptr();
+    width = t.element_size();
+    int64_t last = t.dim();
+    if (last > 0 && t.stride(-1) == 1) width *= t.size(--last);
+    for (int64_t i = 0; i < last; ++i) {
+      if (t.size(i) == 1) continue;
+      const int64_t stride = t.stride(i) * t.element_size();
+      if (stride == 0) {
+        twice = true;
+        continue;
+      }
+      axes.push_back({stride, t.size(i)});
+      reach += stride * (t.size(i) - 1);
+    }
+  }
+};
+
+// Whether two tensors share a byte: whether a run of b starts less than a run's length before or behind one
+// of a.  The distance of two starts is a sum of multiples of the strides; the largest stride is
+// chosen first, and only those multiples from which the smaller ones can still come near 0.  Axes
+// nested in each other leave two or three of them an axis.  A search past `budget` steps (strides that do not nest, in
+// tensors that reach over each other) counts as shared.
+struct Meeting {
+  struct Step {
+    int64_t stride, lo, hi, rest_lo, rest_hi;    // multiples lo .. hi; what the steps behind it add
+  };
+  c10::SmallVector<Step, 12> steps;
+  int64_t below, above;            // a distance d is too near for below < d < above
+  bool itself;                     // one tensor: a run does not meet itself
+  int budget = 1 << 15;
+
+  Meeting(const Runs& a, const Runs& b, bool itself_) : below(-b.width), above(a.width), itself(itself_) {
+    for (const Runs::Axis& x : a.axes) add(x.stride, 1 - x.size, 0);
+    for (const Runs::Axis& x : b.axes) add(x.stride, 0, x.size - 1);
+    std::sort(steps.begin(), steps.end(), [](const Step& p, const Step& q) { return p.stride > q.stride; });
+    int64_t lo = 0, hi = 0;
+    for (size_t i = steps.size(); i-- > 0;) {
+      steps[i].rest_lo = lo;
+      steps[i].rest_hi = hi;
+      lo += steps[i].stride * steps[i].lo;
+      hi += steps[i].stride * steps[i].hi;
+    }
+  }
+  void add(int64_t stride, int64_t lo, int64_t hi) {
+    for (Step& s : steps)
+      if (s.stride == stride) {
+        s.lo += lo;
+        s.hi += hi;
+        return;
+      }
+    steps.push_back({stride, lo, hi, 0, 0});
+  }
+  static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+  bool search(size_t at, int64_t d, bool zero) {
+    if (--budget < 0) return true;
+    if (at == steps.size()) return below < d && d < above && !(itself && zero);
+    const Step& s = steps[at];
+    const int64_t lo = std::max(s.lo, floor_div(below - d - s.rest_hi, s.stride) + 1);
+    const int64_t hi = std::min(s.hi, -floor_div(d + s.rest_lo - above, s.stride) - 1);
+    for (int64_t m = lo; m <= hi; ++m)
+      if (search(at + 1, d + m * s.stride, zero && m == 0)) return true;
+    return false;
+  }
+};
+
+bool meet(const Runs& a, const Runs& b) {
+  if (a.width == 0 || b.width == 0) return false;
+  const int64_t d = (int64_t)(b.begin - a.begin);
+  if (d >= a.reach + a.width || -d >= b.reach + b.width) return false;
+  return Meeting(a, b, false).search(0, d, false);
+}
+
+// a result's memory: no element twice, and what it reads either element for element in the same place or
+// elsewhere
 void apart(const at::Tensor& out, const at::Tensor& in, const char* name, const char* what) {
-  if (at::has_internal_overlap(out) == at::MemOverlap::Yes)
+  const Runs o(out);
+  if (o.width == 0) return;
+  // (in one tensor two equal strides would cancel in the difference: they hold an element twice)
+  bool twice = o.twice;
+  for (size_t i = 1; i < o.axes.size(); ++i)
+    for (size_t j = 0; j < i; ++j) twice = twice || o.axes[i].stride == o.axes[j].stride;
+  if (twice || (!out.is_contiguous() && Meeting(o, o, true).search(0, 0, true)))
     refuse(what, ": ", name, " must not hold an element twice (strides ", out.strides(), ")");
-  const bool same = out.data_ptr() == in.data_ptr() && out.strides() == in.strides();
-  if (!same && at::get_overlap_status(out, in) == at::MemOverlapStatus::Partial)
-    refuse(what, ": ", name, " overlaps an input without being it");
+  bool same = out.data_ptr() == in.data_ptr();
+  for (int64_t i = 0; same && i < out.dim(); ++i)
+    same = out.size(i) == 1 || out.stride(i) == in.stride(i);
+  if (!same && meet(o, Runs(in))) refuse(what, ": ", name, " overlaps an input without being it");
 }
 
 // a result's memory against what it must not touch at all
 void disjoint(const at::Tensor& out, std::initializer_list<const at::Tensor*> others, const char* name,
               const char* what) {
-  for (const at::Tensor* o : others) {
-    if (o == nullptr || !o->defined()) continue;
-    const auto s = at::get_overlap_status(out, *o);
-    if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial)
+  const Runs r(out);
+  for (const at::Tensor* o : others)
+    if (o != nullptr && o->defined() && meet(r, Runs(*o)))
       refuse(what, ": ", name, " overlaps another tensor of the call");
-  }
 }
 
 // ---- rows: the leading axes folded to (outer, inner) ------------------------------------------

@@ -884,7 +884,8 @@ def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dent
     """d loss / d logits from d loss / d log_prob and d loss / d entropy ([..] float32, either may be
     None); `forward` is what categorical_log_prob returned for the same logits, actions, mask,
     temperature and first_action.  Masked actions and padding rows get 0.  The result has the logits'
-    type; `out` may be the logits' own tensor (else it must not overlap them)."""
+    type; `out` may be the logits' own tensor, else no element of it may be one of the call's other
+    tensors (slices that lie between each other's rows or columns are fine)."""
     return (_token_ops or _bind()).categorical_log_prob_backward(
         logits, actions, forward.entropy, forward.stats, dlog_prob, dentropy, mask, temperature,
         first_action, out)
@@ -917,7 +918,7 @@ def layer_norm_forward(x, gamma, beta, epsilon=1e-3, out=None, stats=None):
     """keras LayerNormalization over the last axis: (x - mean) / sqrt(var + epsilon) * gamma + beta
     (csrc/layer_norm.hip).  x [.., n] float32 / bfloat16 / float16; gamma, beta float32 [n] or None.
     Returns (y, stats): y in x's type, stats [.., 2] float32 (mean, 1 / sqrt(var + epsilon)) for the
-    backward call.  `out` may be x."""
+    backward call.  `out` may be x, else no element of it may be one of the call's other tensors."""
     return (_token_ops or _bind()).layer_norm_forward(x, gamma, beta, epsilon, out, stats)
 
 
@@ -926,7 +927,8 @@ def layer_norm_backward(dy, x, gamma, stats, dx=None, dgamma=None, dbeta=None, m
     """Gradient of layer_norm_forward: (dx, dgamma, dbeta), dx in x's type, the others float32 [n]
     (overwritten; given buffers are filled).  `mask_act`: dx is multiplied by that activation's
     derivative, x being its output (as dense_dx's).  param_grads=False / input_grad=False leave out
-    the weights' / the input's gradient (None in the result).  `dx` may be x or dy."""
+    the weights' / the input's gradient (None in the result).  `dx` may be x or dy, else no element of it
+    may be one of the call's other tensors."""
     return (_token_ops or _bind()).layer_norm_backward(
         dy, x, gamma, stats, dx, dgamma, dbeta, ACT[mask_act], bool(param_grads), bool(input_grad))
 
