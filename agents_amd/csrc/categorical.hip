@@ -172,12 +172,16 @@ __device__ static inline bool cat_allowed(const void* mask, int64_t at) {
   return true;
 }
 
+// a row's index of an action; negative: a padding row
 __device__ static inline int64_t cat_action(const CatArgs& a, int64_t row) {
   if (a.actions == nullptr) return 0;
   const int64_t at = vt_row(row, a.inner, a.a_outer, a.a_inner);
   const int64_t v = a.action_bytes == 8 ? reinterpret_cast<const int64_t*>(a.actions)[at]
                                         : (int64_t)reinterpret_cast<const int32_t*>(a.actions)[at];
-  return v - a.first_action;
+  // (compared first: the difference may need a 65th bit)
+  if (v < a.first_action) return -1;
+  const uint64_t index = (uint64_t)v - (uint64_t)a.first_action;
+  return index < (uint64_t)a.vocab ? (int64_t)index : (int64_t)a.vocab;
 }
 
 // the action's logit, -inf where it is masked (read before the row, so that nothing waits for it)

@@ -1,0 +1,35 @@
+"""Actions of categorical_log_prob whose distance from `first_action` does not fit 64 bits, against the
+float64 statement (oracle/categorical.py) with the mathematical index."""
+import numpy as np
+import pytest
+import torch
+
+from agents_amd import ops
+from oracle import categorical as ocat
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("vocab", [5, 600, 9000])
+def test_indexes_that_do_not_fit(dev, vocab, dtype):
+    """An action's index is its mathematical one: past the end NaN, below 0 padding, however far."""
+    low, high = torch.iinfo(dtype).min, torch.iinfo(dtype).max
+    logits = torch.randn(4, vocab, generator=torch.Generator().manual_seed(3)).to(dev)
+    g = torch.ones(4, device=dev)
+    for first in (-7, 7, -2 ** 62, 2 ** 62, -2 ** 63, 2 ** 63 - 1):
+        values = [low, high, min(max(first, low), high), 0]
+        actions = torch.tensor(values, dtype=dtype, device=dev)
+        index = np.array([min(max(v - first, -1), vocab) for v in values])
+        r = ops.categorical_log_prob(logits, actions, first_action=first)
+        want, en, *_ = ocat.forward(logits.double().cpu().numpy(), index)
+        lp = r.log_prob.double().cpu().numpy()
+        np.testing.assert_array_equal(np.isnan(lp), np.isnan(want))
+        np.testing.assert_array_equal(lp[index < 0], 0.0)
+        # (values below 6 in size; sums of at most 9000 / 64 + 80 roundings)
+        fin = np.isfinite(want)
+        assert np.all(np.abs(lp - want)[fin] <= 300 * U)
+        d = ops.categorical_log_prob_backward(logits, actions, r, g, first_action=first)
+        assert d[torch.from_numpy(index < 0)].eq(0).all() and d[torch.from_numpy(index >= vocab)].isnan().all()
