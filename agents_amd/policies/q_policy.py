@@ -48,9 +48,11 @@ class Categorical:
 
     def most_likely(self, k):
         """(actions [B, k] int64, log-probabilities [B, k]) by descending probability, equal ones by
-        ascending action; k is cut to the number of actions."""
+        ascending action; k is cut to the number of actions.  Where fewer actions have a probability:
+        -1 with log-probability -inf (NaN in a row with NaN); a spec may hold the action -1, so the
+        log-probability tells the two apart."""
         r = ops.categorical_log_prob(self.logits, top_k=k)
-        return r.top_ids + self._policy._lo, r.top_log_prob
+        return torch.where(r.top_ids < 0, r.top_ids, r.top_ids + self._policy._lo), r.top_log_prob
 
 
 def distribution_of(policy, time_step, temperature):
