@@ -27,11 +27,14 @@ def _action_bounds(action_spec):
 class Categorical:
     """What `policy.distribution(time_step).action` exposes of tfp Categorical: `logits` [B, A],
     `mode()` (first arg-max, greedy_policy.py:70-89), `log_prob(actions)` and `entropy()` [B], and the
-    most likely actions (`most_likely`)."""
+    most likely actions (`most_likely`).  Actions that `mask` [B, A] excludes are -FLT_MAX in `logits`
+    (q_policy.py:150-194) and have probability 0: log_prob -inf, never among the most likely ones.  A
+    row that excludes every action has no distribution: log_prob -inf, entropy 0."""
 
-    def __init__(self, logits, policy):
+    def __init__(self, logits, policy, mask=None):
         self.logits = logits
         self._policy = policy
+        self._mask = mask
 
     def mode(self):
         return self._policy.select(self.logits, None, 0.0)
@@ -40,18 +43,18 @@ class Categorical:
         """Log-probabilities of actions of the policy's action spec: [B] int32 / int64, or [B, 1] for
         a spec of shape (1,)."""
         r = ops.categorical_log_prob(self.logits, actions.reshape(self.logits.shape[0]),
-                                     first_action=self._policy._lo)
+                                     mask=self._mask, first_action=self._policy._lo)
         return r.log_prob
 
     def entropy(self):
-        return ops.categorical_log_prob(self.logits).entropy
+        return ops.categorical_log_prob(self.logits, mask=self._mask).entropy
 
     def most_likely(self, k):
         """(actions [B, k] int64, log-probabilities [B, k]) by descending probability, equal ones by
         ascending action; k is cut to the number of actions.  Where fewer actions have a probability:
         -1 with log-probability -inf (NaN in a row with NaN); a spec may hold the action -1, so the
         log-probability tells the two apart."""
-        r = ops.categorical_log_prob(self.logits, top_k=k)
+        r = ops.categorical_log_prob(self.logits, mask=self._mask, top_k=k)
         return torch.where(r.top_ids < 0, r.top_ids, r.top_ids + self._policy._lo), r.top_log_prob
 
 
@@ -72,12 +75,13 @@ def distribution_of(policy, time_step, temperature):
         q = policy._q_values(obs, B, dev)
         logits = torch.empty_like(q)
         if mask is not None:
-            mask = mask.to(torch.int32).contiguous()
+            # a copy: the distribution reads it later, and the observation's buffer may be written again
+            mask = mask.to(torch.int32, copy=True, memory_format=torch.contiguous_format)
         _lib.check(_lib.load().aa_boltzmann_action(
             q.data_ptr(), None if mask is None else mask.data_ptr(), B, policy._num_actions,
             float(temperature), None, 0, None, None, policy._lo, None, 0, logits.data_ptr(), 0,
             _lib.stream_ptr()), "aa_boltzmann_action")
-    return policy_step.PolicyStep(Categorical(logits, policy), (), ())
+    return policy_step.PolicyStep(Categorical(logits, policy, mask), (), ())
 
 
 class _DiscretePolicy(tf_policy.TFPolicy):

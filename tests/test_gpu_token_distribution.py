@@ -41,6 +41,43 @@ def close(got, want):
     assert np.all(np.abs(got[fin] - want[fin]) <= 100 * U)
 
 
+@pytest.mark.parametrize("lo", [2, 0, -3])
+@pytest.mark.parametrize("temperature", [None, 0.5, 3.0])
+def test_excluded_actions_have_no_probability(dev, lo, temperature):
+    policy, net = make_policy(lo, lo + 4)
+    x = torch.randn(5, 3, generator=torch.Generator().manual_seed(0)).to(dev)
+    mask = torch.tensor([[1, 1, 1, 1, 1], [0, 0, 0, 1, 0], [1, 0, 0, 0, 1], [0, 1, 0, 0, 0],
+                         [0, 0, 0, 0, 0]], dtype=torch.int32, device=dev)
+    p = policy if temperature is None else boltzmann_policy.BoltzmannPolicy(policy, temperature)
+    dist = p.distribution(ts.restart({"x": x, "mask": mask}, batch_size=5)).action
+    q, m = net.forward(x).double().cpu().numpy(), mask.cpu().numpy()
+    for a in range(5):
+        actions = np.full(5, a)
+        lp, en, ids, top, _ = ocat.forward(q, actions, m, temperature or 1.0, 4)
+        close(dist.log_prob(torch.from_numpy(actions + lo).to(dev)), lp)
+    close(dist.entropy(), en)
+    got_ids, got_top = dist.most_likely(4)
+    np.testing.assert_array_equal(got_ids.cpu().numpy(), np.where(ids < 0, ids, ids + lo))
+    close(got_top, top)
+    # the most likely action is the mode wherever there is one
+    assert torch.equal(got_ids[:4, 0], dist.mode()[:4])
+
+
+def test_the_mask_is_the_one_of_the_time_step(dev):
+    """An observation buffer that is written again does not change a distribution."""
+    policy, net = make_policy(0, 4)
+    x = torch.randn(2, 3, generator=torch.Generator().manual_seed(1)).to(dev)
+    mask = torch.tensor([[1, 0, 1, 0, 1], [0, 1, 1, 0, 0]], dtype=torch.int32, device=dev)
+    dist = policy.distribution(ts.restart({"x": x, "mask": mask}, batch_size=2)).action
+    before = dist.most_likely(5) + (dist.entropy(), dist.log_prob(torch.tensor([1, 1], device=dev)))
+    x.zero_()
+    mask.fill_(1)
+    after = dist.most_likely(5) + (dist.entropy(), dist.log_prob(torch.tensor([1, 1], device=dev)))
+    for a, b in zip(before, after):
+        assert torch.equal(a, b)
+    assert float(before[3][0]) == -INF and (before[0][1, 2:] == -1).all()
+
+
 @pytest.mark.parametrize("lo", [2, -3])
 def test_no_alternative_is_no_action(dev, lo):
     """The marker of a missing alternative is -1 whatever the spec's minimum."""
