@@ -124,9 +124,9 @@ class CategoricalDesc(Structure):
                 ("a_outer", c_int64), ("a_inner", c_int64), ("first_action", c_int64),
                 ("mask", c_void_p), ("k_outer", c_int64), ("k_inner", c_int64),
                 ("dtype", c_int32), ("action_bytes", c_int32), ("mask_bytes", c_int32),
-                ("top_k", c_int32), ("temperature", c_float), ("log_prob", c_void_p),
-                ("entropy", c_void_p), ("stats", c_void_p), ("top_ids", c_void_p),
-                ("top_log_prob", c_void_p)]
+                ("top_k", c_int32), ("temperature", c_float), ("no_padding", c_int32),
+                ("log_prob", c_void_p), ("entropy", c_void_p), ("stats", c_void_p),
+                ("top_ids", c_void_p), ("top_log_prob", c_void_p)]
 
 
 class LayerNormDesc(Structure):

@@ -44,7 +44,7 @@ struct CatArgs {
   int vocab;
   const void* logits; int64_t x_outer, x_inner;
   const void* actions; int64_t a_outer, a_inner, first_action;
-  int action_bytes;
+  int action_bytes, no_padding;
   const void* mask; int64_t k_outer, k_inner;
   float inv_t;                     // 1 / temperature
   int top_k;
@@ -179,7 +179,7 @@ __device__ static inline int64_t cat_action(const CatArgs& a, int64_t row) {
   const int64_t v = a.action_bytes == 8 ? reinterpret_cast<const int64_t*>(a.actions)[at]
                                         : (int64_t)reinterpret_cast<const int32_t*>(a.actions)[at];
   // (compared first: the difference may need a 65th bit)
-  if (v < a.first_action) return -1;
+  if (v < a.first_action) return a.no_padding ? (int64_t)a.vocab : -1;
   const uint64_t index = (uint64_t)v - (uint64_t)a.first_action;
   return index < (uint64_t)a.vocab ? (int64_t)index : (int64_t)a.vocab;
 }
@@ -723,7 +723,7 @@ static CatArgs cat_args(const aa_categorical_desc* d) {
   a.rows = d->rows; a.inner = d->inner; a.vocab = (int)d->vocab;
   a.logits = d->logits; a.x_outer = d->x_outer; a.x_inner = d->x_inner;
   a.actions = d->actions; a.a_outer = d->a_outer; a.a_inner = d->a_inner;
-  a.first_action = d->first_action; a.action_bytes = d->action_bytes;
+  a.first_action = d->first_action; a.action_bytes = d->action_bytes; a.no_padding = d->no_padding;
   a.mask = d->mask; a.k_outer = d->k_outer; a.k_inner = d->k_inner;
   a.inv_t = 1.f / d->temperature; a.top_k = d->top_k;
   a.log_prob = d->log_prob; a.entropy = d->entropy; a.stats = d->stats;

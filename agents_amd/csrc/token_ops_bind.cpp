@@ -396,7 +396,7 @@ struct Categorical {
 };
 
 Categorical categorical_args(PyObject* logits, PyObject* actions, PyObject* mask, PyObject* temperature,
-                             PyObject* first_action, const char* what) {
+                             PyObject* first_action, PyObject* padding, const char* what) {
   Categorical c;
   const at::Tensor& x = tensor_given(logits, what, "logits");
   c.logits = &x;
@@ -446,6 +446,7 @@ Categorical categorical_args(PyObject* logits, PyObject* actions, PyObject* mask
   d.action_bytes = c.actions != nullptr ? (int32_t)c.actions->element_size() : 4;
   d.mask_bytes = c.mask.defined() ? (int32_t)c.mask.element_size() : 1;
   d.temperature = (float)t;
+  d.no_padding = padding != Py_True;
   return c;
 }
 
@@ -461,13 +462,13 @@ Fold categorical_fold(Categorical& c, const at::Tensor* out, const char* what) {
   return f[3];
 }
 
-// (logits, actions, mask, temperature, top_k, first_action)
+// (logits, actions, mask, temperature, top_k, first_action, padding)
 //   -> (log_prob, entropy, top_ids, top_log_prob, stats)
 PyObject* py_categorical(PyObject*, PyObject* const* a, Py_ssize_t n) {
   AA_BIND_BEGIN
   const char* what = "categorical_log_prob";
-  count(n, 6, what);
-  Categorical c = categorical_args(a[0], a[1], a[2], a[3], a[5], what);
+  count(n, 7, what);
+  Categorical c = categorical_args(a[0], a[1], a[2], a[3], a[5], a[6], what);
   int64_t k = whole(a[4], what, "top_k");
   if (k < 0 || k > AA_CATEGORICAL_MAX_TOP)
     refuse(what, ": top_k must be 0..", AA_CATEGORICAL_MAX_TOP, ", got ", k);
@@ -502,13 +503,13 @@ PyObject* py_categorical(PyObject*, PyObject* const* a, Py_ssize_t n) {
   AA_BIND_END
 }
 
-// (logits, actions, entropy, stats, dlog_prob, dentropy, mask, temperature, first_action, out)
+// (logits, actions, entropy, stats, dlog_prob, dentropy, mask, temperature, first_action, padding, out)
 //   -> dlogits
 PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   AA_BIND_BEGIN
   const char* what = "categorical_log_prob_backward";
-  count(n, 10, what);
-  Categorical c = categorical_args(a[0], a[1], a[6], a[7], a[8], what);
+  count(n, 11, what);
+  Categorical c = categorical_args(a[0], a[1], a[6], a[7], a[8], a[9], what);
   const at::Tensor& x = *c.logits;
   const auto lead = lead_of(x);
   const at::Tensor& entropy = tensor_given(a[2], what, "forward.entropy");
@@ -533,7 +534,7 @@ PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !stats.is_contiguous())
     refuse(what, ": forward.stats is not of these logits");
   at::Tensor out;
-  const at::Tensor* const o = tensor(a[9], what, "out");
+  const at::Tensor* const o = tensor(a[10], what, "out");
   if (o != nullptr) {
     if (o->scalar_type() != x.scalar_type() || o->sizes() != x.sizes() || !last_contiguous(*o))
       refuse(what, ": out must be ", x.scalar_type(), " ", x.sizes(),

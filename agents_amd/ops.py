@@ -862,33 +862,34 @@ CategoricalLogProb = collections.namedtuple(
     "CategoricalLogProb", ("log_prob", "entropy", "top_ids", "top_log_prob", "stats"))
 
 
-def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k=0, first_action=0):
+def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k=0, first_action=0,
+                         padding=True):
     """Log-probabilities of `actions` under Categorical(logits / temperature), with the entropy and
     the `top_k` most likely alternatives (csrc/categorical.hip).
 
     logits [.., A] float32 / bfloat16 / float16, any strides whose leading axes fold to two; actions
     [..] int32 / int64 (None: entropy and alternatives only); mask broadcastable to logits (its last
     axis A), bool / uint8 / int32, 0 excludes an action.  `actions - first_action` indexes A.  A
-    negative index marks a padding row: log_prob and entropy 0, ids -1, its logits are not used.  An
-    index past the end gives NaN.  A row whose mask leaves no finite logit: log_prob -inf, entropy 0.
+    negative index marks a padding row: log_prob and entropy 0, ids -1, its logits are not used; with
+    padding=False it is out of range.  An index out of range gives NaN.  A row whose mask leaves no finite logit: log_prob -inf, entropy 0.
     Returns CategoricalLogProb: log_prob, entropy [..] float32, top_ids [.., k] int64 and
     top_log_prob [.., k] float32 with k = min(top_k, A) (None for top_k=0; equal logits by lower
     index, -1 / -inf where fewer actions have a probability; ids index A, without first_action), and
     `stats` for the backward call."""
     return CategoricalLogProb(*(_token_ops or _bind()).categorical_log_prob(
-        logits, actions, mask, temperature, top_k, first_action))
+        logits, actions, mask, temperature, top_k, first_action, bool(padding)))
 
 
 def categorical_log_prob_backward(logits, actions, forward, dlog_prob=None, dentropy=None, mask=None,
-                                  temperature=1.0, first_action=0, out=None):
+                                  temperature=1.0, first_action=0, out=None, padding=True):
     """d loss / d logits from d loss / d log_prob and d loss / d entropy ([..] float32, either may be
     None); `forward` is what categorical_log_prob returned for the same logits, actions, mask,
-    temperature and first_action.  Masked actions and padding rows get 0.  The result has the logits'
-    type; `out` may be the logits' own tensor, else no element of it may be one of the call's other
-    tensors (slices that lie between each other's rows or columns are fine)."""
+    temperature, first_action and padding.  Masked actions and padding rows get 0.  The result has the
+    logits' type; `out` may be the logits' own tensor, else no element of it may be one of the call's
+    other tensors (slices that lie between each other's rows or columns are fine)."""
     return (_token_ops or _bind()).categorical_log_prob_backward(
         logits, actions, forward.entropy, forward.stats, dlog_prob, dentropy, mask, temperature,
-        first_action, out)
+        first_action, bool(padding), out)
 
 
 # ---- clipping of many gradient tensors ------------------------------------------------------------

@@ -41,9 +41,10 @@ class Categorical:
 
     def log_prob(self, actions):
         """Log-probabilities of actions of the policy's action spec: [B] int32 / int64, or [B, 1] for
-        a spec of shape (1,)."""
+        a spec of shape (1,).  NaN for an action that is not of the spec, above or below."""
         r = ops.categorical_log_prob(self.logits, actions.reshape(self.logits.shape[0]),
-                                     mask=self._mask, first_action=self._policy._lo)
+                                     mask=self._mask, first_action=self._policy._lo,
+                                     padding=False)
         return r.log_prob
 
     def entropy(self):

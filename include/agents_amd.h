@@ -1081,7 +1081,8 @@ int aa_norm_apply(const float* x, int64_t n_outer, int64_t n_inner, const float*
  * alternatives (tfp Categorical.log_prob / entropy as policies use them; csrc/categorical.hip).
  *   mask [rows, vocab] (nullable; bytes or int32, 0 excludes an action: probability 0 exactly).
  *   action index = actions[r] - first_action.  Negative: a padding row -- log_prob, entropy and
- *   gradient are 0, its logits are not used.  Past the end: log_prob and gradient are NaN.
+ *   gradient are 0, its logits are not used; with no_padding it is out of range like an index past the
+ *   end, whose log_prob and gradient are NaN.
  *   A row without any allowed finite logit: log_prob -inf, entropy 0, gradient 0.  NaN or +inf in an
  *   allowed place: NaN.
  *   top_k <= AA_CATEGORICAL_MAX_TOP (and <= vocab): ids (without first_action) and log-probabilities
@@ -1098,6 +1099,7 @@ typedef struct aa_categorical_desc {
   int64_t k_outer, k_inner;
   int32_t dtype, action_bytes /* 4 or 8 */, mask_bytes /* 1 or 4 */, top_k;
   float temperature;            /* 1e-30 .. 1e30 */
+  int32_t no_padding;           /* 0: negative indexes are padding rows */
   float* log_prob;              /* [rows] */
   float* entropy;               /* [rows], nullable */
   float* stats;                 /* [rows][2], nullable in the forward call */

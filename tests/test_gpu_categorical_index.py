@@ -33,3 +33,21 @@ def test_indexes_that_do_not_fit(dev, vocab, dtype):
         assert np.all(np.abs(lp - want)[fin] <= 300 * U)
         d = ops.categorical_log_prob_backward(logits, actions, r, g, first_action=first)
         assert d[torch.from_numpy(index < 0)].eq(0).all() and d[torch.from_numpy(index >= vocab)].isnan().all()
+
+
+@pytest.mark.parametrize("vocab", [5, 600, 9000, 20001])
+def test_without_padding(dev, vocab):
+    """padding=False: an index below 0 is out of range like one past the end; the others are as before."""
+    logits = torch.randn(6, vocab, generator=torch.Generator().manual_seed(5)).to(dev)
+    actions = torch.tensor([3, 2, 4, vocab + 2, vocab + 3, 0], device=dev)
+    bad = torch.tensor([False, True, False, False, True, True], device=dev)
+    g, h = torch.ones(6, device=dev), torch.full((6,), 0.5, device=dev)
+    r = ops.categorical_log_prob(logits, actions, first_action=3, padding=False, top_k=3)
+    d = ops.categorical_log_prob_backward(logits, actions, r, g, h, first_action=3, padding=False)
+    assert torch.equal(r.log_prob.isnan(), bad) and d[bad].isnan().all()
+    inside = torch.where(bad, 3, actions)
+    want = ops.categorical_log_prob(logits, inside, first_action=3, top_k=3)
+    wd = ops.categorical_log_prob_backward(logits, inside, want, g, h, first_action=3)
+    assert torch.equal(r.log_prob[~bad], want.log_prob[~bad]) and torch.equal(d[~bad], wd[~bad])
+    # what does not depend on the action is the row's own
+    assert torch.equal(r.entropy, want.entropy) and torch.equal(r.top_ids, want.top_ids)

@@ -89,3 +89,15 @@ def test_no_alternative_is_no_action(dev, lo):
     ids, top = dist.most_likely(3)
     assert ids.tolist() == [[-1, -1, -1], [lo + 1, lo + 4, -1], [-1, -1, -1]]
     assert top[0].isnan().all() and float(top[1, 2]) == -INF and (top[2] == -INF).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("lo", [2, -3])
+def test_actions_outside_the_spec(dev, lo, dtype):
+    policy, net = make_policy(lo, lo + 4, dtype, masked=False)
+    low, high = torch.iinfo(dtype).min, torch.iinfo(dtype).max
+    actions = torch.tensor([lo, lo - 1, lo - 2, low, lo + 4, lo + 5, high, low + 2], dtype=dtype, device=dev)
+    x = torch.randn(len(actions), 3, generator=torch.Generator().manual_seed(2)).to(dev)
+    dist = policy.distribution(ts.restart(x, batch_size=len(actions))).action
+    want, *_ = ocat.forward(net.forward(x).double().cpu().numpy(), np.array([0, 9, 9, 9, 4, 9, 9, 9]))
+    close(dist.log_prob(actions), want)
