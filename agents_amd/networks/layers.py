@@ -91,7 +91,7 @@ def get_initializer(x, default):
     if isinstance(x, Initializer):
         return x
     if isinstance(x, str):
-        return {"zeros": Zeros(), "glorot_uniform": GlorotUniform(),
+        return {"zeros": Zeros(), "ones": Constant(1.0), "glorot_uniform": GlorotUniform(),
                 "orthogonal": Orthogonal()}[x]
     raise TypeError(f"unsupported initializer {x!r}")
 
