@@ -562,15 +562,16 @@ PyObject* py_categorical_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- clipping ---------------------------------------------------------------------------------
-// items of a sequence of tensors; `hold` owns the sequence while they are used
+// items of a sequence of tensors; `hold`, a tuple of the call's own, keeps them while they are used (the
+// caller's list may change meanwhile: a number's conversion is Python code, a launch lets other threads run)
 std::vector<const at::Tensor*> tensors(PyObject* o, PyObject** hold, const char* what,
                                        const char* name) {
-  *hold = PySequence_Fast(o, "a list of tensors is needed");
+  *hold = PySequence_Tuple(o);
   if (*hold == nullptr) throw Raised{};
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(*hold);
+  const Py_ssize_t n = PyTuple_GET_SIZE(*hold);
   std::vector<const at::Tensor*> ts((size_t)n);
   for (Py_ssize_t i = 0; i < n; ++i)
-    ts[i] = &tensor_given(PySequence_Fast_GET_ITEM(*hold, i), what, name);
+    ts[i] = &tensor_given(PyTuple_GET_ITEM(*hold, i), what, name);
   return ts;
 }
 
@@ -653,7 +654,7 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   PyObject* out = nullptr;     // owned; released on every way out but the last
   Held out_guard;
   if (!os.empty()) {
-    out = out_guard.o = PySequence_List(a[4]);
+    out = out_guard.o = PySequence_List(hold_out.o);
     if (out == nullptr) throw Raised{};
   } else if (scale) {
     int64_t total = 0;
