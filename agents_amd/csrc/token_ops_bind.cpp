@@ -653,13 +653,20 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   for (size_t i = 0; i < n; ++i) on_device({&t0, ts[i], os.empty() ? nullptr : os[i]});
   PyObject* out = nullptr;     // owned; released on every way out but the last
   Held out_guard;
+  // The scratch, some kilobytes of sums, lies behind the clipped tensors (an allocation less); the norm is
+  // one of its own, so that a program that keeps the norm of every step keeps no more than that.
+  const int64_t need = lib.clip_bytes(sizes.data(), (int32_t)n);
+  at::Tensor sums;
+  void* ws = nullptr;
   if (!os.empty()) {
     out = out_guard.o = PySequence_List(hold_out.o);
     if (out == nullptr) throw Raised{};
   } else if (scale) {
     int64_t total = 0;
-    for (size_t i = 0; i < n; ++i) total += Pieces::room(sizes[i], t0.element_size());
-    Pieces pieces(total, t0.options());
+    const int64_t width = t0.element_size();
+    for (size_t i = 0; i < n; ++i) total += Pieces::room(sizes[i], width);
+    Pieces pieces(total + (need + width - 1) / width, t0.options());
+    ws = static_cast<char*>(pieces.flat.data_ptr()) + total * width;
     out = out_guard.o = PyList_New((Py_ssize_t)n);
     if (out == nullptr) throw Raised{};
     for (size_t i = 0; i < n; ++i) {
@@ -671,12 +678,11 @@ PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     out = out_guard.o = Py_None;
     Py_INCREF(out);
   }
-  // (the scratch, some kilobytes of sums, behind the norms)
-  const int64_t need = lib.clip_bytes(sizes.data(), (int32_t)n);
-  const int64_t norms = each ? (int64_t)n : 1;
-  Pieces small(Pieces::room(norms, 4) + (need + 3) / 4, f32(t0));
-  const at::Tensor norm = each ? small.take({norms}) : small.take({});
-  void* const ws = static_cast<float*>(small.flat.data_ptr()) + small.at;
+  if (ws == nullptr) {
+    sums = scratch(need, t0);
+    ws = data(sums);
+  }
+  const at::Tensor norm = each ? at::empty({(int64_t)n}, f32(t0)) : at::empty({}, f32(t0));
   {
     OnDevice on(t0);
     check(unlocked(lib.clip, src.data(), scale ? dst.data() : nullptr, sizes.data(), (int32_t)n,
