@@ -873,7 +873,7 @@ def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k
     negative index marks a padding row: log_prob and entropy 0, ids -1, its logits are not used; with
     padding=False it is out of range.  An index out of range gives NaN.  A row whose mask leaves no finite logit: log_prob -inf, entropy 0.
     Returns CategoricalLogProb: log_prob, entropy [..] float32, top_ids [.., k] int64 and
-    top_log_prob [.., k] float32 with k = min(top_k, A) (None for top_k=0; equal logits by lower
+    top_log_prob [.., k] float32 with k = min(top_k, A) (top_k 0 .. 64, None for 0; equal logits by lower
     index, -1 / -inf where fewer actions have a probability; ids index A, without first_action), and
     `stats` for the backward call."""
     return CategoricalLogProb(*(_token_ops or _bind()).categorical_log_prob(

@@ -52,10 +52,12 @@ class Categorical:
 
     def most_likely(self, k):
         """(actions [B, k] int64, log-probabilities [B, k]) by descending probability, equal ones by
-        ascending action; k is cut to the number of actions.  Where fewer actions have a probability:
+        ascending action; k >= 1 is cut to the number of actions and may be 64 at most then.  Where fewer actions have a probability:
         -1 with log-probability -inf (NaN in a row with NaN); a spec may hold the action -1, so the
         log-probability tells the two apart."""
-        r = ops.categorical_log_prob(self.logits, mask=self._mask, top_k=k)
+        if k < 1:
+            raise ValueError(f"most_likely: k must be at least 1, got {k}")
+        r = ops.categorical_log_prob(self.logits, mask=self._mask, top_k=min(k, self.logits.shape[1]))
         return torch.where(r.top_ids < 0, r.top_ids, r.top_ids + self._policy._lo), r.top_log_prob
 
 

@@ -101,3 +101,22 @@ def test_actions_outside_the_spec(dev, lo, dtype):
     dist = policy.distribution(ts.restart(x, batch_size=len(actions))).action
     want, *_ = ocat.forward(net.forward(x).double().cpu().numpy(), np.array([0, 9, 9, 9, 4, 9, 9, 9]))
     close(dist.log_prob(actions), want)
+
+
+def test_how_many_alternatives(dev):
+    """More than there are actions: all of them; none at all is refused, 64 of many is the limit."""
+    policy, net = make_policy(2, 6, masked=False)
+    x = torch.randn(2, 3, generator=torch.Generator().manual_seed(2)).to(dev)
+    dist = policy.distribution(ts.restart(x, batch_size=2)).action
+    all_ids, all_top = dist.most_likely(5)
+    for k in (6, 64, 65, 1000):
+        ids, top = dist.most_likely(k)
+        assert torch.equal(ids, all_ids) and torch.equal(top, all_top)
+    for k in (0, -1):
+        with pytest.raises(ValueError, match="at least 1"):
+            dist.most_likely(k)
+    many, _ = make_policy(0, 99, masked=False)
+    dist = many.distribution(ts.restart(x, batch_size=2)).action
+    assert dist.most_likely(64)[0].shape == (2, 64)
+    with pytest.raises(ValueError, match="top_k"):
+        dist.most_likely(65)
