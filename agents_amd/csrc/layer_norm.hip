@@ -12,8 +12,8 @@
 // fixed order (no atomics: same bits every call).  One workgroup of 1,024 lanes per CU: the partials
 // cost a write and a read of 8 bytes a column and workgroup, which at 512 workgroups of 256 lanes was
 // as much as the rows themselves for 2000 rows of 2048.
-// bf16 8192x4096 (67 MB an array): forward 27 .. 30 us, 4.5 .. 5.0 TB/s, backward 40 .. 42 and 4 for the
-// join, 4.5 TB/s; f32 256x512, by latency: 3.5, 5.7 and 2 us.
+// bf16 8192x4096 (67 MB an array): forward 28 .. 30 us, 4.5 TB/s, backward 39 .. 42, 5.0 TB/s, and 5 for
+// the join; f32 256x512, by latency: 3.5, 5.7 and 2 us.
 // Rows past 8,192 columns have no registers left for the weights' sums: their columns are summed by a
 // pass of its own; past 16,384 the rows are walked in loops.
 #include <math.h>
@@ -144,7 +144,9 @@ aa_layer_norm_fwd_kernel(LnArgs a) {
   float gm[NCH][C], bt[NCH][C];
   ln_load_weight<C, NCH>(a.gamma, lane, TEAM, a.width, 1.f, gm);
   ln_load_weight<C, NCH>(a.beta, lane, TEAM, a.width, 0.f, bt);
-  // (a quotient, not a product with 1 / D: a constant row's mean is its value, its y is beta)
+  // (A quotient, not a product with 1 / D: one rounding less.  A constant row's y is beta where the sum is
+  // exact, as for 2; else its mean is as far off as the sum of its values, a few 2^-24 of their size, and y by
+  // that over sqrt(epsilon): 1000 columns of 100.1, epsilon 1e-3: mean 1.5e-5, y 4.9e-4 gamma.)
   const float width = (float)a.width;
   for (int64_t base = wave0; base < a.rows; base += stride) {
     const int64_t row = base + ahead;
@@ -257,7 +259,8 @@ template <typename T, int TEAM, int NCH, bool WEIGHTS>
 __global__ void __launch_bounds__(1024) aa_layer_norm_bwd_kernel(LnArgs a) {
   constexpr int C = T::C;
   constexpr int PER = 1024 / TEAM;
-  // gamma and the next row in registers: 128 registers a lane hold them beside the sums of 8 columns
+  // gamma and the next row in registers: 128 registers a lane hold them beside the sums of 8 columns (109 ..
+  // 127 are used; teams of 512 need a few more and leave 9 values in fp16, 3 in fp32, in scratch memory)
   constexpr bool AHEAD = NCH * C <= 8;
   constexpr int COLS = TEAM * NCH * C;           // columns of a team
   constexpr int UNIT = TEAM < 64 ? 64 : TEAM;    // lanes that hold one set of sums at the end
@@ -585,7 +588,8 @@ static int64_t ln_groups(int64_t rows, int64_t width) {
     // row groups of the columns' pass, 32 .. 128: f16 2000x12000 backward 86 us at 64, 71 at 128;
     // f32 200x9000 18 at 64, 21 at 128.  Few rows: one group, which needs no launch to join it (one
     // group | a group a row: f32 4x9001 9.2 | 11.0 us, 4x65536 20 | 29, 16x65536 23 | 34; the other
-    // way round for bf16 8x9001 13.5 | 11.8, 16x16384 15 | 12, 64x65536 68 | 42)
+    // way round for bf16 8x9001 13.5 | 11.8, 16x16384 15 | 12, 64x65536 68 | 42).  Between 16,384 and
+    // 65,536 columns, where the rule goes from 4 rows to 16, nothing was measured, nor a size in both types.
     if (rows <= (width < 65536 ? 4 : 16)) return 1;
     const int64_t want = rows / 8 < 32 ? 32 : rows / 8 > 128 ? 128 : rows / 8;
     return rows < want ? rows : want;
