@@ -10,11 +10,11 @@
 // The alternatives ride in the same pass: a wave keeps its 64 best keys (value, then lower index)
 // sorted across its lanes, a chunk whose maximum stays below the k-th costs one comparison, the others
 // collect in LDS and are merged 64 at a time by a bitonic network.
-// Bound by HBM for vocabularies (268 MB of bf16, 4096x32768: forward 57 .. 59 us, 4.6 TB/s; gradient,
-// which reads and writes them, 82 .. 84 us, 6.4 TB/s; f16 2044x50001, 204 MB, 42 .. 45 and 64 .. 66),
-// by launch and latency for a few actions (f32 4096x18 with an int32 mask: 3.7 and 3.9 us).  Few rows:
+// Bound by HBM for vocabularies (268 MB of bf16, 4096x32768: forward 56 .. 60 us, 4.5 TB/s; gradient,
+// which reads and writes them, 82 .. 85 us, 6.4 TB/s; f16 2044x50001, 204 MB, 43 .. 46 and 64 .. 66),
+// by launch and latency for a few actions (f32 4096x18 with an int32 mask: 3.6 and 4.0 us).  Few rows:
 // a row is split over workgroups and the parts joined by a second launch (bf16 1x131072 with 20
-// alternatives: 8.5 + 4 us).
+// alternatives: 8.8 + 4.2 us).
 #include <math.h>
 #include "common.h"
 #include "agents_amd.h"
@@ -197,6 +197,8 @@ __device__ static inline float cat_action_logit(const CatArgs& a, int64_t row, i
 __device__ static inline float cat_nan() { return __uint_as_float(0x7fc00000u); }
 
 // one lane: everything of a row but its alternatives; returns ln S (+inf: no distribution)
+// (the reference may lie CAT_MARGIN powers of two below the row's maximum, so the value of an action that
+// is all but certain is a difference of two numbers of up to 2.8: off by some 2e-7, on either side of 0)
 __device__ static inline float cat_finish(const CatArgs& a, int64_t row, int64_t action, float x,
                                           CatSum u) {
   const bool empty = u.s == 0.f;
@@ -223,7 +225,8 @@ __device__ static inline void cat_write_top(const CatArgs& a, int64_t row, int l
       real ? (cat_key_value(key) - r) * a.inv_t - ls : isnan(ls) ? ls : -INFINITY;
 }
 
-// a padding row (negative action): nothing of it is read
+// a padding row (negative action): its logits are not used (the first tile of them, for few actions the
+// row, is on its way before the action is known)
 __device__ static inline void cat_pad_row(const CatArgs& a, int64_t row, int lane) {
   if (lane == 0) {
     a.log_prob[row] = 0.f;

@@ -9,8 +9,8 @@
 // float64 -- a square of the float32 range neither overflows nor vanishes there, and an addition in
 // float64 costs no more than one in float32 on this machine --; the pieces' sums are added in a fixed
 // order by every workgroup of the second pass itself (at most a few thousand of them, from L2), so
-// the join costs no launch.  14 bf16 tensors of 333 MB: 57 .. 59 us (5.7 TB/s) and 108 .. 110 (6.1); 10
-// f32 tensors of 7 MB: 4 and 5.  Past AA_CLIP_JOIN pieces a launch of one workgroup adds them first.
+// the join costs no launch.  14 bf16 tensors of 333 MB: 56 .. 58 us (5.8 TB/s) and 108 .. 110 (6.1); 10
+// f32 tensors of 7 MB: 4.1 and 5.7.  Past AA_CLIP_JOIN pieces a launch of one workgroup adds them first.
 #include <math.h>
 #include "common.h"
 #include "agents_amd.h"

@@ -847,6 +847,8 @@ def dense_loss_head_ok(B, A, mask_src):
 
 
 # ---- policies over many discrete actions (tokens) ---------------------------------------------
+# Results lie outside torch's autograd graph, whether or not an input requires a gradient: gradients are
+# what the backward calls return (`logits.backward(dlogits)` hands one to a graph that made the logits).
 # Checks, outputs, strides and scratch of these operators are compiled (csrc/token_ops_bind.cpp):
 # in Python they cost several times what the kernels of a small call take.
 _token_ops = None
@@ -871,11 +873,14 @@ def categorical_log_prob(logits, actions=None, mask=None, temperature=1.0, top_k
     [..] int32 / int64 (None: entropy and alternatives only); mask broadcastable to logits (its last
     axis A), bool / uint8 / int32, 0 excludes an action.  `actions - first_action` indexes A.  A
     negative index marks a padding row: log_prob and entropy 0, ids -1, its logits are not used; with
-    padding=False it is out of range.  An index out of range gives NaN.  A row whose mask leaves no finite logit: log_prob -inf, entropy 0.
+    padding=False it is out of range.  An index out of range gives NaN.  A row whose mask leaves no finite
+    logit: log_prob -inf, entropy 0.  float32 arithmetic: next to 0 a log-probability is off by some
+    2e-7 and may lie above it, an entropy below.
     Returns CategoricalLogProb: log_prob, entropy [..] float32, top_ids [.., k] int64 and
-    top_log_prob [.., k] float32 with k = min(top_k, A) (top_k 0 .. 64, None for 0; equal logits by lower
-    index, -1 / -inf where fewer actions have a probability; ids index A, without first_action), and
-    `stats` for the backward call."""
+    top_log_prob [.., k] float32 with k = min(top_k, A) (top_k 0 .. 64, None for 0; equal logits by
+    lower index, -1 / -inf where fewer actions have a probability; ids index A, without first_action),
+    and `stats` for the backward call.  The float32 results are pieces of one allocation, which lives as
+    long as any of them: clone what is kept for long."""
     return CategoricalLogProb(*(_token_ops or _bind()).categorical_log_prob(
         logits, actions, mask, temperature, top_k, first_action, bool(padding)))
 
@@ -926,7 +931,7 @@ def layer_norm_forward(x, gamma, beta, epsilon=1e-3, out=None, stats=None):
 def layer_norm_backward(dy, x, gamma, stats, dx=None, dgamma=None, dbeta=None, mask_act=None,
                         param_grads=True, input_grad=True):
     """Gradient of layer_norm_forward: (dx, dgamma, dbeta), dx in x's type, the others float32 [n]
-    (overwritten; given buffers are filled).  `mask_act`: dx is multiplied by that activation's
+    (overwritten; given buffers are filled, others are pieces of one allocation).  `mask_act`: dx is multiplied by that activation's
     derivative, x being its output (as dense_dx's).  param_grads=False / input_grad=False leave out
     the weights' / the input's gradient (None in the result).  `dx` may be x or dy, else no element of it
     may be one of the call's other tensors."""
