@@ -259,7 +259,7 @@ template <typename T, int TEAM, int NCH, bool WEIGHTS>
 __global__ void __launch_bounds__(1024) aa_layer_norm_bwd_kernel(LnArgs a) {
   constexpr int C = T::C;
   constexpr int PER = 1024 / TEAM;
-  // gamma and the next row in registers: 128 registers a lane hold them beside the sums of 8 columns (109 ..
+  // gamma and the next row in registers: 128 registers a lane hold them beside the sums of 8 columns (110 ..
   // 127 are used; teams of 512 need a few more and leave 9 values in fp16, 3 in fp32, in scratch memory)
   constexpr bool AHEAD = NCH * C <= 8;
   constexpr int COLS = TEAM * NCH * C;           // columns of a team

@@ -145,9 +145,9 @@ struct Runs {
 };
 
 // Whether two tensors share a byte: whether a run of b starts less than a run's length before or behind one
-// of a.  The distance of two starts is a sum of multiples of the strides; the largest stride is
-// chosen first, and only those multiples from which the smaller ones can still come near 0.  Axes
-// nested in each other leave two or three of them an axis.  A search past `budget` steps (strides that do not nest, in
+// of a.  The distance of two starts is a sum of multiples of the strides; the largest stride is chosen
+// first, and only those multiples from which the smaller ones can still come near 0.  Axes nested in each
+// other leave two or three of them an axis.  A search past `budget` steps (strides that do not nest, in
 // tensors that reach over each other) counts as shared.
 struct Meeting {
   struct Step {

@@ -931,10 +931,10 @@ def layer_norm_forward(x, gamma, beta, epsilon=1e-3, out=None, stats=None):
 def layer_norm_backward(dy, x, gamma, stats, dx=None, dgamma=None, dbeta=None, mask_act=None,
                         param_grads=True, input_grad=True):
     """Gradient of layer_norm_forward: (dx, dgamma, dbeta), dx in x's type, the others float32 [n]
-    (overwritten; given buffers are filled, others are pieces of one allocation).  `mask_act`: dx is multiplied by that activation's
-    derivative, x being its output (as dense_dx's).  param_grads=False / input_grad=False leave out
-    the weights' / the input's gradient (None in the result).  `dx` may be x or dy, else no element of it
-    may be one of the call's other tensors."""
+    (overwritten; given buffers are filled, others are pieces of one allocation).  `mask_act`: dx is
+    multiplied by that activation's derivative, x being its output (as dense_dx's).  param_grads=False /
+    input_grad=False leave out the weights' / the input's gradient (None in the result).  `dx` may be x
+    or dy, else no element of it may be one of the call's other tensors."""
     return (_token_ops or _bind()).layer_norm_backward(
         dy, x, gamma, stats, dx, dgamma, dbeta, ACT[mask_act], bool(param_grads), bool(input_grad))
 
