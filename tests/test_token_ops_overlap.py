@@ -11,7 +11,7 @@ from agents_amd import _lib, ops
 pytestmark = pytest.mark.usefixtures("lib")
 
 
-def verdict(fn, *a, **kw):
+def outcome(fn, *a, **kw):
     """"overlaps", "twice", or "" for a call that passes every check but the one for device tensors."""
     try:
         fn(*a, **kw)
@@ -27,21 +27,21 @@ def verdict(fn, *a, **kw):
 
 
 def norm_over(x, out):
-    return verdict(ops.layer_norm_forward, x, None, None, out=out)
+    return outcome(ops.layer_norm_forward, x, None, None, out=out)
 
 
 def grad_over(x, out):
     a = torch.zeros(x.shape[:-1], dtype=torch.int64)
     r = ops.CategoricalLogProb(None, torch.zeros(x.shape[:-1]), None, None, torch.zeros(*x.shape[:-1], 2))
-    return verdict(ops.categorical_log_prob_backward, x, a, r, torch.zeros(x.shape[:-1]), out=out)
+    return outcome(ops.categorical_log_prob_backward, x, a, r, torch.zeros(x.shape[:-1]), out=out)
 
 
 def dx_over(x, out):
-    return verdict(ops.layer_norm_backward, torch.zeros(x.shape), x, None, torch.zeros(*x.shape[:-1], 2), dx=out)
+    return outcome(ops.layer_norm_backward, torch.zeros(x.shape), x, None, torch.zeros(*x.shape[:-1], 2), dx=out)
 
 
 def dx_over_dy(dy, out):
-    return verdict(ops.layer_norm_backward, dy, torch.zeros(dy.shape), None, torch.zeros(*dy.shape[:-1], 2), dx=out)
+    return outcome(ops.layer_norm_backward, dy, torch.zeros(dy.shape), None, torch.zeros(*dy.shape[:-1], 2), dx=out)
 
 
 CALLS = [norm_over, grad_over, dx_over, dx_over_dy]
@@ -140,26 +140,26 @@ def test_other_tensors_of_the_call():
     rows = flat.as_strided((4, 10), (20, 1))                     # room between the rows
     w_between, w_inside = flat[10:20], flat[15:25]
     f = ops.layer_norm_forward
-    assert verdict(f, x, w_between, None, out=rows) == ""
-    assert verdict(f, x, None, w_between, out=rows) == ""
-    assert verdict(f, x, w_inside, None, out=rows) == "overlaps"
-    assert verdict(f, x, None, w_inside, out=rows) == "overlaps"
-    assert verdict(f, rows, None, None, stats=flat[10:18].view(4, 2)) == ""
-    assert verdict(f, rows, None, None, stats=flat[14:22].view(4, 2)) == "overlaps"
+    assert outcome(f, x, w_between, None, out=rows) == ""
+    assert outcome(f, x, None, w_between, out=rows) == ""
+    assert outcome(f, x, w_inside, None, out=rows) == "overlaps"
+    assert outcome(f, x, None, w_inside, out=rows) == "overlaps"
+    assert outcome(f, rows, None, None, stats=flat[10:18].view(4, 2)) == ""
+    assert outcome(f, rows, None, None, stats=flat[14:22].view(4, 2)) == "overlaps"
     g, st = ops.layer_norm_backward, torch.zeros(4, 2)
-    assert verdict(g, x, rows, None, st, dgamma=w_between) == ""
-    assert verdict(g, x, rows, None, st, dgamma=w_inside) == "overlaps"
-    assert verdict(g, rows, x, None, st, dbeta=w_inside) == "overlaps"
-    assert verdict(g, x, x, None, st, dx=rows, dbeta=w_inside) == "overlaps"
+    assert outcome(g, x, rows, None, st, dgamma=w_between) == ""
+    assert outcome(g, x, rows, None, st, dgamma=w_inside) == "overlaps"
+    assert outcome(g, rows, x, None, st, dbeta=w_inside) == "overlaps"
+    assert outcome(g, x, x, None, st, dx=rows, dbeta=w_inside) == "overlaps"
     a = torch.zeros(4, dtype=torch.int64)
     r = ops.CategoricalLogProb(None, torch.zeros(4), None, None, st)
     b = ops.categorical_log_prob_backward
-    assert verdict(b, x, a, r, flat[10:14], out=rows) == ""
-    assert verdict(b, x, a, r, flat[18:22], out=rows) == "overlaps"
-    assert verdict(b, x, a, r._replace(stats=flat[58:66].view(4, 2)), torch.zeros(4), out=rows) == "overlaps"
+    assert outcome(b, x, a, r, flat[10:14], out=rows) == ""
+    assert outcome(b, x, a, r, flat[18:22], out=rows) == "overlaps"
+    assert outcome(b, x, a, r._replace(stats=flat[58:66].view(4, 2)), torch.zeros(4), out=rows) == "overlaps"
     ints = flat.view(torch.int64)                                # (places 5 .. 9 lie between two rows)
-    assert verdict(b, x, ints[5:9], r, torch.zeros(4), out=rows) == ""
-    assert verdict(b, x, ints[7:11], r, torch.zeros(4), out=rows) == "overlaps"
+    assert outcome(b, x, ints[5:9], r, torch.zeros(4), out=rows) == ""
+    assert outcome(b, x, ints[7:11], r, torch.zeros(4), out=rows) == "overlaps"
     mask = flat.view(torch.int32).as_strided((4, 10), (20, 1), 10)
-    assert verdict(b, x, a, r, torch.zeros(4), mask=mask, out=rows) == ""
-    assert verdict(b, x, a, r, torch.zeros(4), mask=flat.view(torch.int32)[15:25], out=rows) == "overlaps"
+    assert outcome(b, x, a, r, torch.zeros(4), mask=mask, out=rows) == ""
+    assert outcome(b, x, a, r, torch.zeros(4), mask=flat.view(torch.int32)[15:25], out=rows) == "overlaps"
